@@ -276,6 +276,112 @@ int rt_get_xcd_shares(rt_ctx* ctx, double* shares8);
  * roundtrip.py:57) and roundtrip_amd/checkpoint.py verifies through this.  Host code, needs no context or GPU. */
 uint32_t rt_crc32c(const void* data, size_t n, uint32_t crc);
 
+/* --- Network blocks -----------------------------------------------------------------------------------------------------
+ * The layers deep networks put around and between plain dense ones, next to rt_mlp_forward_dev: a gated feed-forward block
+ * and the norms before and after it, forward and backward.  NO COUNTERPART IN THE REFERENCE (its networks are chains of
+ * dense layers, model.py:61-88).
+ *   - all pointers in the structs are DEVICE pointers to arrays of the call's dtype, rows contiguous; an ld* is the distance
+ *     of two rows in elements (0: rows are dense), at most 2^20.  Nothing needs more alignment than its elements have;
+ *     arrays whose rows start on 16 bytes and are whole multiples of 16 bytes long are read fastest.
+ *   - the sums of products, the norms' sums and everything between two stores are float32 or wider; a stored value is rounded
+ *     once, to nearest even.
+ *   - calls enqueue on the context's stream and return; they allocate nothing and keep nothing.  What they need beyond their
+ *     arguments is the caller's workspace (device memory aligned to 16 bytes, contents irrelevant before and after), so a
+ *     call can be captured into a graph (rt_ctx_stream).  Calls of one context are ordered, and may share a workspace; give
+ *     graphs that may run at the same time a workspace each.
+ *   - an output may not share memory with an input or another output, except where a function says so (columns of one
+ *     buffer with equal ld* do not share memory).  Rows and columns outside the arrays' extents are neither read nor written.
+ *   - results do not depend on what else runs, and a call repeated gives the same bits (no floating-point atomics).
+ *   - the device that was current stays current. */
+#define RT_F32  0
+#define RT_BF16 1
+#define RT_F16  2
+
+#define RT_ACT_SILU      0   /* g / (1 + exp(-g)) */
+#define RT_ACT_GELU_TANH 1   /* 0.5 g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) */
+#define RT_ACT_LRELU     2   /* g > 0 ? g : alpha g   (the framework's own; alpha = 0: ReLU); derivative 1 for g > 0, else alpha */
+#define RT_ACT_SIGMOID   3   /* 1 / (1 + exp(-g)) */
+
+#define RT_NORM_RMS   0      /* v / sqrt(mean(v^2) + eps) */
+#define RT_NORM_LAYER 1      /* the same of v - mean(v) */
+
+/* The stream the context enqueues on (a hipStream_t), for callers that order other work against it or capture its calls
+ * into a graph.  It stays the context's: do not destroy it. */
+int rt_ctx_stream(rt_ctx* ctx, void** stream);
+
+/* out = h w_down,  h = act(x w_gate) * (x w_up)      T rows; widths and strides up to 2^20, T up to 2^40 */
+typedef struct rt_gated_ffn {
+    int32_t dtype, act;          /* RT_F32 / RT_BF16 / RT_F16;  RT_ACT_* */
+    int32_t d_in, d_ff, d_out;
+    float   alpha;               /* RT_ACT_LRELU */
+    int64_t T;                   /* 0: nothing to do (gradients of weights: zeros) */
+    int64_t ldx, ld_in, ld_down, ld_out, ld_pre;
+    const void *x;               /* T x d_in */
+    const void *w_gate, *w_up;   /* d_in x d_ff, both with stride ld_in */
+    const void *w_down;          /* d_ff x d_out */
+    void *out;                   /* T x d_out */
+    void *pre_gate, *pre_up;     /* T x d_ff: x w_gate and x w_up, kept for the backward pass; both NULL if there is none */
+} rt_gated_ffn;
+
+/* Gradients of sum(dout * out).  A NULL output is not computed. */
+typedef struct rt_gated_ffn_grads {
+    int64_t ld_dout, ld_dx, ld_dw_in, ld_dw_down;
+    const void *dout;            /* T x d_out */
+    void *dx;                    /* T x d_in */
+    void *dw_gate, *dw_up;       /* d_in x d_ff, both with stride ld_dw_in */
+    void *dw_down;               /* d_ff x d_out */
+} rt_gated_ffn_grads;
+
+/* Bytes of workspace rt_gated_ffn_dev (backward = 0) or rt_gated_ffn_backward_dev (1) needs for these sizes (pointers and
+ * strides are not looked at): T x d_ff values, three times that backward, and the partial sums of products whose K is split. */
+int rt_gated_ffn_workspace(rt_ctx* ctx, const rt_gated_ffn* args, int backward, size_t* bytes);
+
+/* Forward.  h is rounded to the call's dtype on its way into the second product, as every operand of a matrix instruction is. */
+int rt_gated_ffn_dev(rt_ctx* ctx, const rt_gated_ffn* args, void* ws, size_t ws_bytes);
+
+/* Backward, at the x, weights, pre_gate and pre_up of a forward call (out is not read):
+ *   dh = dout w_down^T;  dg = dh * u * act'(g);  du = dh * act(g)      (rounded to the dtype on their way into the products)
+ *   dx = dg w_gate^T + du w_up^T;  dw_gate = x^T dg;  dw_up = x^T du;  dw_down = h^T dout */
+int rt_gated_ffn_backward_dev(rt_ctx* ctx, const rt_gated_ffn* args, const rt_gated_ffn_grads* grads, void* ws, size_t ws_bytes);
+
+/* y = res_scale x + branch_scale gate * N(branch; w_post)        n = N(y; w_pre)
+ * N(v; w) = RT_NORM_*(v) * (w + w_offset); a NULL w counts as ones, without the offset.  Without a branch y = res_scale x
+ * (the norm before a block: x and n alone).  Row t uses row t / rows_per_gate of gate: 1 is a gate for every row, T one for
+ * all, a sequence length one for each sequence (the last group may be short); a NULL gate counts as ones.
+ * n is made of the unrounded y. */
+typedef struct rt_block_norm {
+    int32_t dtype, kind;         /* RT_NORM_* */
+    int32_t d;                   /* 1 .. 32768 (RT_F32: 16384) */
+    float   eps, res_scale, branch_scale, w_offset;
+    int64_t T;                   /* < 2^31 */
+    int64_t rows_per_gate;
+    int64_t ldx, ld_branch, ldy, ldn, ld_gate;
+    const void *x;               /* T x d */
+    const void *branch;          /* T x d or NULL */
+    const void *gate;            /* ceil(T / rows_per_gate) x d or NULL */
+    const void *w_post, *w_pre;  /* d or NULL */
+    void *y, *n;                 /* T x d; one of them may be NULL; each may be x's or branch's own memory, row for row */
+} rt_block_norm;
+
+/* Gradients of sum(dy * y) + sum(dn * n).  dy or dn may be NULL (zeros); a NULL output is not computed. */
+typedef struct rt_block_norm_grads {
+    int64_t ld_dy, ld_dn, ld_dx, ld_dbranch, ld_dgate;
+    const void *dy, *dn;         /* T x d */
+    void *dx;                    /* T x d; may be y's, dy's or dn's own memory, row for row */
+    void *dbranch;               /* T x d; may be branch's, y's, dy's or dn's own memory, row for row */
+    void *dgate;                 /* gate's shape: the sum over the rows that share it */
+    void *dw_post, *dw_pre;      /* d */
+} rt_block_norm_grads;
+
+/* Bytes of workspace of rt_block_norm_backward_dev (the forward pass needs none). */
+int rt_block_norm_workspace(rt_ctx* ctx, const rt_block_norm* args, size_t* bytes);
+int rt_block_norm_dev(rt_ctx* ctx, const rt_block_norm* args);
+
+/* Backward, at the branch, y, gate and weights of a forward call; x and n are not read (without a branch and without a y, x
+ * is read in y's place). */
+int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_block_norm_grads* grads, void* ws,
+                               size_t ws_bytes);
+
 /* --- Device memory for callers of the *_dev entry points (the reference keeps its arrays in numpy and feeds TF
  * placeholders, main_density_est.py:232,247; a host program that wants its query points resident in HBM needs no other
  * GPU library than this one).  rt_dev_free waits for the context's stream first; the copies are synchronous. */

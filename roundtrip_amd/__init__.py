@@ -5,7 +5,8 @@ Drop-in for the IS path of the reference (`estimate_py_with_IS`, /root/reference
 librt_is.so (hand-written gfx950 HIP kernels behind the C ABI of include/rt_is.h).
 """
 __version__ = '0.1.0'
+from ._lib import Engine
 from .nets import BaseFullyConnectedNet, DenseNet, Generator
 from .roundtrip import Roundtrip, RoundtripModel
 
-__all__ = ['Roundtrip', 'RoundtripModel', 'BaseFullyConnectedNet', 'Generator', 'DenseNet']
+__all__ = ['Roundtrip', 'RoundtripModel', 'BaseFullyConnectedNet', 'Generator', 'DenseNet', 'Engine']

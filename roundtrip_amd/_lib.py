@@ -25,18 +25,52 @@ SYMBOLS = (
     "rt_comm_unique_id", "rt_comm_init", "rt_comm_destroy", "rt_comm_info", "rt_comm_all_gather_f64",
     "rt_comm_all_gather_f64_dev", "rt_comm_all_reduce_max_f64", "rt_comm_barrier",
     "rt_is_kernel_name", "rt_cf_estimate", "rt_cf_estimate_dev", "rt_mean_stderr", "rt_mean_stderr_dev", "rt_is_estimate_summary",
+    "rt_ctx_stream", "rt_gated_ffn_workspace", "rt_gated_ffn_dev", "rt_gated_ffn_backward_dev",
+    "rt_block_norm_workspace", "rt_block_norm_dev", "rt_block_norm_backward_dev",
 )
 
+RT_EINVAL = 1
+RT_EUNSUPPORTED = 4
 RT_ETOOBIG = 6
 RT_ECOMM = 7
 RT_EBUSY = 8
 RT_NOALLOC_SCRATCH_BYTES = 32 << 20
 RT_COMM_ID_BYTES = 128
 
+RT_F32, RT_BF16, RT_F16 = 0, 1, 2
+RT_ACT_SILU, RT_ACT_GELU_TANH, RT_ACT_LRELU, RT_ACT_SIGMOID = 0, 1, 2, 3
+RT_NORM_RMS, RT_NORM_LAYER = 0, 1
+
 
 class RtCounters(C.Structure):
     _fields_ = [("kernel_ms", C.c_double), ("flops", C.c_double), ("launches", C.c_uint64),
                 ("sample_evals", C.c_uint64)]
+
+
+class RtGatedFfn(C.Structure):
+    """rt_gated_ffn (include/rt_is.h): one gated feed-forward block in device memory.  Kept by the caller and used as often
+    as the addresses in it hold."""
+    _fields_ = ([(k, C.c_int32) for k in ("dtype", "act", "d_in", "d_ff", "d_out")] + [("alpha", C.c_float)]
+                + [(k, C.c_int64) for k in ("T", "ldx", "ld_in", "ld_down", "ld_out", "ld_pre")]
+                + [(k, C.c_void_p) for k in ("x", "w_gate", "w_up", "w_down", "out", "pre_gate", "pre_up")])
+
+
+class RtGatedFfnGrads(C.Structure):
+    _fields_ = ([(k, C.c_int64) for k in ("ld_dout", "ld_dx", "ld_dw_in", "ld_dw_down")]
+                + [(k, C.c_void_p) for k in ("dout", "dx", "dw_gate", "dw_up", "dw_down")])
+
+
+class RtBlockNorm(C.Structure):
+    """rt_block_norm (include/rt_is.h): the norms before and after a block, with its gate and residual, in device memory."""
+    _fields_ = ([(k, C.c_int32) for k in ("dtype", "kind", "d")]
+                + [(k, C.c_float) for k in ("eps", "res_scale", "branch_scale", "w_offset")]
+                + [(k, C.c_int64) for k in ("T", "rows_per_gate", "ldx", "ld_branch", "ldy", "ldn", "ld_gate")]
+                + [(k, C.c_void_p) for k in ("x", "branch", "gate", "w_post", "w_pre", "y", "n")])
+
+
+class RtBlockNormGrads(C.Structure):
+    _fields_ = ([(k, C.c_int64) for k in ("ld_dy", "ld_dn", "ld_dx", "ld_dbranch", "ld_dgate")]
+                + [(k, C.c_void_p) for k in ("dy", "dn", "dx", "dbranch", "dgate", "dw_post", "dw_pre")])
 
 
 class RtError(RuntimeError):
@@ -107,6 +141,13 @@ def load():
     lib.rt_mean_stderr_dev.argtypes = [vp, vp, i64, vp]
     lib.rt_is_estimate_summary.argtypes = [vp, vp, vp, i64, i64, i64, dbl, dbl, dbl, C.c_uint64, vp, C.POINTER(dbl),
                                            C.POINTER(dbl)]
+    lib.rt_ctx_stream.argtypes = [vp, C.POINTER(vp)]
+    lib.rt_gated_ffn_workspace.argtypes = [vp, C.POINTER(RtGatedFfn), C.c_int, C.POINTER(C.c_size_t)]
+    lib.rt_gated_ffn_dev.argtypes = [vp, C.POINTER(RtGatedFfn), vp, C.c_size_t]
+    lib.rt_gated_ffn_backward_dev.argtypes = [vp, C.POINTER(RtGatedFfn), C.POINTER(RtGatedFfnGrads), vp, C.c_size_t]
+    lib.rt_block_norm_workspace.argtypes = [vp, C.POINTER(RtBlockNorm), C.POINTER(C.c_size_t)]
+    lib.rt_block_norm_dev.argtypes = [vp, C.POINTER(RtBlockNorm)]
+    lib.rt_block_norm_backward_dev.argtypes = [vp, C.POINTER(RtBlockNorm), C.POINTER(RtBlockNormGrads), vp, C.c_size_t]
     for name in SYMBOLS:
         fn = getattr(lib, name)
         if name not in ("rt_last_error", "rt_crc32c"):
@@ -339,6 +380,73 @@ class Engine(object):
         self._chk(self._lib.rt_is_estimate_dev_noalloc(self._h, y_ptr, xhat_ptr, int(N), int(y_index_base),
                                                        int(sample_size), float(sd_y), float(scale), float(df),
                                                        int(seed), int(bool(log)), out_ptr))
+
+    # ---- network blocks: gated feed-forward and the norms around it (rt_gated_ffn*, rt_block_norm*) ----
+    # An *_args / *_grads struct describes a call by raw device addresses (None: absent), sizes and row strides in elements
+    # (0: dense); its fields can be changed between calls.  Calls enqueue on the engine's stream.
+    F32, BF16, F16 = RT_F32, RT_BF16, RT_F16
+    SILU, GELU_TANH, LRELU, SIGMOID = RT_ACT_SILU, RT_ACT_GELU_TANH, RT_ACT_LRELU, RT_ACT_SIGMOID
+    RMS, LAYER = RT_NORM_RMS, RT_NORM_LAYER
+
+    @property
+    def stream(self):
+        """The hipStream_t the engine enqueues on, as an integer (e.g. for torch.cuda.ExternalStream)."""
+        p = C.c_void_p()
+        self._chk(self._lib.rt_ctx_stream(self._h, C.byref(p)))
+        return p.value
+
+    @staticmethod
+    def gated_ffn_args(T, d_in, d_ff, d_out, dtype, act, x=None, w_gate=None, w_up=None, w_down=None, out=None,
+                       pre_gate=None, pre_up=None, alpha=0.2, ldx=0, ld_in=0, ld_down=0, ld_out=0, ld_pre=0):
+        """out = (act(x w_gate) * (x w_up)) w_down; pre_gate / pre_up keep what the backward pass needs."""
+        return RtGatedFfn(dtype=dtype, act=act, d_in=d_in, d_ff=d_ff, d_out=d_out, alpha=alpha, T=T, ldx=ldx, ld_in=ld_in,
+                          ld_down=ld_down, ld_out=ld_out, ld_pre=ld_pre, x=x, w_gate=w_gate, w_up=w_up, w_down=w_down,
+                          out=out, pre_gate=pre_gate, pre_up=pre_up)
+
+    @staticmethod
+    def gated_ffn_grads(dout=None, dx=None, dw_gate=None, dw_up=None, dw_down=None, ld_dout=0, ld_dx=0, ld_dw_in=0,
+                        ld_dw_down=0):
+        return RtGatedFfnGrads(ld_dout=ld_dout, ld_dx=ld_dx, ld_dw_in=ld_dw_in, ld_dw_down=ld_dw_down, dout=dout, dx=dx,
+                               dw_gate=dw_gate, dw_up=dw_up, dw_down=dw_down)
+
+    def gated_ffn_workspace(self, args, backward=False):
+        """Bytes of device memory a forward (or backward) call on these sizes needs beside its arrays."""
+        n = C.c_size_t()
+        self._chk(self._lib.rt_gated_ffn_workspace(self._h, C.byref(args), int(bool(backward)), C.byref(n)))
+        return int(n.value)
+
+    def gated_ffn_dev(self, args, ws_ptr=None, ws_bytes=0):
+        self._chk(self._lib.rt_gated_ffn_dev(self._h, C.byref(args), ws_ptr, ws_bytes))
+
+    def gated_ffn_backward_dev(self, args, grads, ws_ptr=None, ws_bytes=0):
+        self._chk(self._lib.rt_gated_ffn_backward_dev(self._h, C.byref(args), C.byref(grads), ws_ptr, ws_bytes))
+
+    @staticmethod
+    def block_norm_args(T, d, dtype, kind, x=None, branch=None, y=None, n=None, w_post=None, w_pre=None, gate=None,
+                        rows_per_gate=1, res_scale=1.0, branch_scale=1.0, eps=1e-5, w_offset=0.0, ldx=0, ld_branch=0, ldy=0,
+                        ldn=0, ld_gate=0):
+        """y = res_scale x + branch_scale gate * N(branch; w_post), n = N(y; w_pre)."""
+        return RtBlockNorm(dtype=dtype, kind=kind, d=d, eps=eps, res_scale=res_scale, branch_scale=branch_scale,
+                           w_offset=w_offset, T=T, rows_per_gate=rows_per_gate, ldx=ldx, ld_branch=ld_branch, ldy=ldy, ldn=ldn,
+                           ld_gate=ld_gate, x=x, branch=branch, gate=gate, w_post=w_post, w_pre=w_pre, y=y, n=n)
+
+    @staticmethod
+    def block_norm_grads(dy=None, dn=None, dx=None, dbranch=None, dgate=None, dw_post=None, dw_pre=None, ld_dy=0, ld_dn=0,
+                         ld_dx=0, ld_dbranch=0, ld_dgate=0):
+        return RtBlockNormGrads(ld_dy=ld_dy, ld_dn=ld_dn, ld_dx=ld_dx, ld_dbranch=ld_dbranch, ld_dgate=ld_dgate, dy=dy, dn=dn,
+                                dx=dx, dbranch=dbranch, dgate=dgate, dw_post=dw_post, dw_pre=dw_pre)
+
+    def block_norm_workspace(self, args):
+        """Bytes of device memory a backward call on these sizes needs beside its arrays (forward: none)."""
+        n = C.c_size_t()
+        self._chk(self._lib.rt_block_norm_workspace(self._h, C.byref(args), C.byref(n)))
+        return int(n.value)
+
+    def block_norm_dev(self, args):
+        self._chk(self._lib.rt_block_norm_dev(self._h, C.byref(args)))
+
+    def block_norm_backward_dev(self, args, grads, ws_ptr=None, ws_bytes=0):
+        self._chk(self._lib.rt_block_norm_backward_dev(self._h, C.byref(args), C.byref(grads), ws_ptr, ws_bytes))
 
     # ---- device memory (rt_dev_alloc & co.): what callers of the *_dev entry points keep their arrays in ----
     def dev_alloc(self, nbytes):

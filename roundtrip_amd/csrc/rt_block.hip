@@ -1,0 +1,643 @@
+// rt_block.hip — the network-block operators of the C ABI: the gated feed-forward block and the norms around it, forward and
+// backward (include/rt_is.h).  Kernels: rt_gemm.hpp (matrix cores), rt_norm.hpp (memory bound).
+//
+// Every call is a few launches on the context's stream, allocates nothing and keeps nothing: what it needs beyond its
+// arguments is the caller's workspace.  So a call can be captured into a graph, and two graphs do not meet unless their
+// caller gives them the same workspace.
+
+#include "rt_internal.hpp"
+#include <math.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <string.h>
+
+namespace {
+
+#include "rt_gemm.hpp"
+#include "rt_norm.hpp"
+
+int failf(rt_ctx* ctx, int code, const char* fmt, ...) {
+    char msg[320];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(msg, sizeof msg, fmt, ap);
+    va_end(ap);
+    return rt_ctx_fail(ctx, code, msg);
+}
+
+#define HIPCHK(ctx, call)                                                                          \
+    do {                                                                                           \
+        const hipError_t e_ = (call);                                                              \
+        if (e_ != hipSuccess) return failf(ctx, RT_EHIP, "%s: %s", #call, hipGetErrorString(e_));  \
+    } while (0)
+
+// Makes the context's device current for the duration of a call, and what was current again behind it.
+struct DeviceScope {
+    int before = -1;
+    hipError_t err;
+    explicit DeviceScope(int device) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+        else before = -1;
+    }
+    ~DeviceScope() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+constexpr int64_t MAX_DIM = 1 << 20;              // elements of a row, and of its stride: a tile then spans < 2^31 bytes
+constexpr int64_t MAX_ROWS = 1ll << 40;
+
+int elem_size(int dtype) { return dtype == RT_F32 ? 4 : 2; }
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// A strided matrix in device memory, as the checks see it.
+struct Mat {
+    const char* name;
+    const void* p;
+    int64_t rows, width, ld;      // ld in elements
+};
+
+// Whether two matrices share an element.  Columns of one buffer (equal strides, disjoint column ranges) do not.
+bool overlap(const Mat& a, const Mat& b, int es) {
+    if (!a.p || !b.p || a.rows == 0 || b.rows == 0) return false;
+    const uintptr_t a0 = (uintptr_t)a.p, a1 = a0 + ((a.rows - 1) * a.ld + a.width) * es;
+    const uintptr_t b0 = (uintptr_t)b.p, b1 = b0 + ((b.rows - 1) * b.ld + b.width) * es;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (a.ld != b.ld) return true;
+    const int64_t pitch = a.ld * es, d = (int64_t)(b0 - a0) % pitch, off = d < 0 ? d + pitch : d;
+    return !(off >= a.width * es && off + b.width * es <= pitch);
+}
+
+bool same_place(const Mat& a, const Mat& b) { return a.p == b.p && (a.ld == b.ld || a.rows <= 1); }
+
+int check_mat(rt_ctx* ctx, const char* fn, const Mat& m, int es, bool required) {
+    if (!m.p) return required && m.rows > 0 ? failf(ctx, RT_EINVAL, "%s: %s is NULL", fn, m.name) : RT_OK;
+    if ((uintptr_t)m.p % es) return failf(ctx, RT_EINVAL, "%s: %s is not aligned to its %d-byte elements", fn, m.name, es);
+    if (m.ld < m.width)
+        return failf(ctx, RT_EINVAL, "%s: the row stride of %s (%lld) is less than its width (%lld)", fn, m.name, (long long)m.ld,
+                     (long long)m.width);
+    if (m.ld > MAX_DIM)
+        return failf(ctx, RT_EUNSUPPORTED, "%s: the row stride of %s (%lld) exceeds %lld", fn, m.name, (long long)m.ld,
+                     (long long)MAX_DIM);
+    return RT_OK;
+}
+
+// No output may share memory with an input or another output.
+int check_disjoint(rt_ctx* ctx, const char* fn, const Mat* in, int nin, const Mat* out, int nout, int es) {
+    for (int i = 0; i < nout; ++i) {
+        for (int j = 0; j < nin; ++j)
+            if (overlap(out[i], in[j], es)) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, in[j].name);
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j], es)) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, out[j].name);
+    }
+    return RT_OK;
+}
+
+int check_ws(rt_ctx* ctx, const char* fn, const void* ws, size_t have, size_t need) {
+    if (need == 0) return RT_OK;
+    if (!ws) return failf(ctx, RT_EINVAL, "%s: workspace is NULL (%zu bytes needed)", fn, need);
+    if ((uintptr_t)ws % 16) return failf(ctx, RT_EINVAL, "%s: workspace is not aligned to 16 bytes", fn);
+    if (have < need) return failf(ctx, RT_EINVAL, "%s: workspace of %zu bytes, %zu needed", fn, have, need);
+    return RT_OK;
+}
+
+// ---- matrix products ----------------------------------------------------------------------------------------------
+struct Product {                // C [M x N] = X W over K, nseg segments, nbatch products side by side
+    int lx, lw, epi;
+    int64_t M, K;
+    int N, nseg, nbatch;
+};
+
+struct Plan {
+    int bm, bn, splits, per_split, nk, tiles_m, tiles_n, nslot, Np;
+    size_t part_bytes;
+};
+
+int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, Plan& pl) {
+    const int ke = 128 / elem_size(dtype);
+    pl.bm = pl.bn = 128;
+    const int cn = p.epi == EPI_GATED ? pl.bn / 2 : pl.bn;
+    const int64_t tm = (p.M + pl.bm - 1) / pl.bm, tn = (p.N + cn - 1) / cn, nk = (p.K + ke - 1) / ke;
+    if (tm * tn > 0x7fffffff || nk * p.nseg > 0x7fffffff)
+        return failf(ctx, RT_EUNSUPPORTED, "a product of %lld x %d over %lld is larger than one launch covers", (long long)p.M, p.N,
+                     (long long)p.K);
+    pl.tiles_m = (int)tm;
+    pl.tiles_n = (int)tn;
+    pl.nk = (int)nk;
+    pl.nslot = p.epi == EPI_GATED ? 2 : p.nbatch;
+    pl.Np = (int)up(p.N, 4);
+    const int64_t tiles = tm * tn * p.nbatch, steps = nk * p.nseg;
+    int64_t s = tiles >= cus ? 1 : cus / tiles;
+    if (s > steps / 4) s = steps / 4;
+    if (s < 1) s = 1;
+    pl.per_split = (int)((steps + s - 1) / s);
+    pl.splits = (int)((steps + pl.per_split - 1) / pl.per_split);
+    pl.part_bytes = pl.splits > 1 ? (size_t)pl.splits * pl.nslot * p.M * pl.Np * sizeof(float) : 0;
+    return RT_OK;
+}
+
+// One row for each kernel that a product can run on.
+typedef void (*GemmFn)(GemmArgs);
+template <int DT, int LX, int LW, int EPI>
+GemmFn gemm_fn(bool al) {
+    return al ? gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, true> : gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, false>;
+}
+
+template <int DT>
+int launch_product(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a, bool al) {
+    a.M = p.M; a.N = p.N; a.K = p.K; a.nseg = p.nseg; a.nk = pl.nk;
+    a.tiles_m = pl.tiles_m; a.tiles_n = pl.tiles_n;
+    a.splits = pl.splits; a.per_split = pl.per_split; a.Np = pl.Np; a.nslot = pl.nslot;
+    GemmFn fn, join;
+    if (p.epi == EPI_GATED) {
+        fn = gemm_fn<DT, LK, LI, EPI_GATED>(al);
+        join = gemm_join_kernel<DT, EPI_GATED>;
+    } else if (p.epi == EPI_GATED_BWD) {
+        fn = gemm_fn<DT, LK, LK, EPI_GATED_BWD>(al);
+        join = gemm_join_kernel<DT, EPI_GATED_BWD>;
+    } else {
+        fn = p.lx == LI ? gemm_fn<DT, LI, LI, EPI_STORE>(al)
+                        : p.lw == LI ? gemm_fn<DT, LK, LI, EPI_STORE>(al) : gemm_fn<DT, LK, LK, EPI_STORE>(al);
+        join = gemm_join_kernel<DT, EPI_STORE>;
+    }
+    hipLaunchKernelGGL(fn, dim3(pl.tiles_m * pl.tiles_n, pl.splits, p.nbatch), dim3(256), 0, st, a);
+    HIPCHK(ctx, hipGetLastError());
+    if (pl.splits > 1) {
+        const int64_t n = (p.M * (pl.Np / 4) + 255) / 256;
+        hipLaunchKernelGGL(join, dim3((unsigned)(n < 8192 ? n : 8192), 1, p.nbatch), dim3(256), 0, st, a);
+        HIPCHK(ctx, hipGetLastError());
+    }
+    return RT_OK;
+}
+
+int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, GemmArgs& a) {
+    Plan pl;
+    const int rc = plan_product(ctx, v.cu_count, dtype, p, pl);
+    if (rc) return rc;
+    const int es = elem_size(dtype), epc = 16 / es;
+    bool al = (p.lx == LK ? p.K : p.M) % epc == 0 && (p.lw == LK ? p.K : p.N) % epc == 0 && a.ldx[0] % 16 == 0 && a.ldw[0] % 16 == 0;
+    for (int i = 0; i < 2; ++i) al = al && (uintptr_t)a.x[i] % 16 == 0 && (uintptr_t)a.w[i] % 16 == 0;
+    if (dtype == RT_F32) return launch_product<RT_F32>(ctx, v.stream, p, pl, a, al);
+    if (dtype == RT_BF16) return launch_product<RT_BF16>(ctx, v.stream, p, pl, a, al);
+    return launch_product<RT_F16>(ctx, v.stream, p, pl, a, al);
+}
+
+// rows x bytes of zeros: a weight gradient of no tokens.
+__global__ void zero_rows_kernel(char* p, long long ld, long long rows, long long width) {
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+        for (long long c = threadIdx.x * 2; c < width; c += blockDim.x * 2) *(unsigned short*)(p + r * ld + c) = 0;
+}
+
+int zero_rows(rt_ctx* ctx, hipStream_t st, void* p, int64_t ld, int64_t rows, int64_t width) {
+    if (!p) return RT_OK;
+    hipLaunchKernelGGL(zero_rows_kernel, dim3((unsigned)(rows < 1024 ? rows : 1024)), dim3(256), 0, st, (char*)p, ld, rows, width);
+    HIPCHK(ctx, hipGetLastError());
+    return RT_OK;
+}
+
+// ---- the gated feed-forward block ---------------------------------------------------------------------------------
+struct Ffn {
+    rt_gated_ffn a;                // with its strides filled in
+    int es;
+    int64_t ldh;                   // elements; h, dgate and dup lie in the workspace
+    size_t h_bytes;
+    Product gated, down;           // forward
+    Product dh, dx, dw_in, dw_down;
+    Plan pl_gated, pl_down, pl_dh, pl_dx, pl_dw_in, pl_dw_down;
+    size_t ws_fwd, ws_bwd;
+};
+
+size_t most(size_t a, size_t b) { return a > b ? a : b; }
+
+int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& f) {
+    if (!in) return failf(ctx, RT_EINVAL, "%s: the arguments are NULL", fn);
+    f.a = *in;
+    rt_gated_ffn& a = f.a;
+    if (a.dtype != RT_F32 && a.dtype != RT_BF16 && a.dtype != RT_F16) return failf(ctx, RT_EINVAL, "%s: unknown dtype %d", fn, a.dtype);
+    if (a.act < RT_ACT_SILU || a.act > RT_ACT_SIGMOID) return failf(ctx, RT_EINVAL, "%s: unknown activation %d", fn, a.act);
+    if (!isfinite(a.alpha)) return failf(ctx, RT_EINVAL, "%s: alpha is not finite", fn);
+    if (a.T < 0 || a.T > MAX_ROWS) return failf(ctx, RT_EINVAL, "%s: T = %lld", fn, (long long)a.T);
+    if (a.d_in < 1 || a.d_ff < 1 || a.d_out < 1 || a.d_in > MAX_DIM || a.d_ff > MAX_DIM || a.d_out > MAX_DIM)
+        return failf(ctx, RT_EINVAL, "%s: widths %d, %d, %d: each must be in [1, %lld]", fn, a.d_in, a.d_ff, a.d_out, (long long)MAX_DIM);
+    f.es = elem_size(a.dtype);
+    if (!a.ldx) a.ldx = a.d_in;
+    if (!a.ld_in) a.ld_in = a.d_ff;
+    if (!a.ld_down) a.ld_down = a.d_out;
+    if (!a.ld_out) a.ld_out = a.d_out;
+    if (!a.ld_pre) a.ld_pre = a.d_ff;
+    f.ldh = up(a.d_ff, 16 / f.es);
+    f.h_bytes = (size_t)up(a.T * f.ldh * f.es, 256);
+    f.gated = {LK, LI, EPI_GATED, a.T, a.d_in, a.d_ff, 1, 1};
+    f.down = {LK, LI, EPI_STORE, a.T, a.d_ff, a.d_out, 1, 1};
+    f.dh = {LK, LK, EPI_GATED_BWD, a.T, a.d_out, a.d_ff, 1, 1};
+    f.dx = {LK, LK, EPI_STORE, a.T, a.d_ff, a.d_in, 2, 1};
+    f.dw_in = {LI, LI, EPI_STORE, a.d_in, a.T, a.d_ff, 1, 2};
+    f.dw_down = {LI, LI, EPI_STORE, a.d_ff, a.T, a.d_out, 1, 1};
+    f.ws_fwd = f.ws_bwd = 0;
+    if (a.T == 0) return RT_OK;
+    int rc;
+    if ((rc = plan_product(ctx, cus, a.dtype, f.gated, f.pl_gated)) || (rc = plan_product(ctx, cus, a.dtype, f.down, f.pl_down)) ||
+        (rc = plan_product(ctx, cus, a.dtype, f.dh, f.pl_dh)) || (rc = plan_product(ctx, cus, a.dtype, f.dx, f.pl_dx)) ||
+        (rc = plan_product(ctx, cus, a.dtype, f.dw_in, f.pl_dw_in)) || (rc = plan_product(ctx, cus, a.dtype, f.dw_down, f.pl_dw_down)))
+        return rc;
+    f.ws_fwd = f.h_bytes + most(f.pl_gated.part_bytes, f.pl_down.part_bytes);
+    f.ws_bwd = 3 * f.h_bytes + most(most(f.pl_dh.part_bytes, f.pl_dx.part_bytes), most(f.pl_dw_in.part_bytes, f.pl_dw_down.part_bytes));
+    return RT_OK;
+}
+
+void set_x(GemmArgs& g, const void* p0, const void* p1, int64_t ld) {
+    g.x[0] = (const char*)p0;
+    g.x[1] = (const char*)p1;
+    g.ldx[0] = g.ldx[1] = ld;
+}
+void set_w(GemmArgs& g, const void* p0, const void* p1, int64_t ld) {
+    g.w[0] = (const char*)p0;
+    g.w[1] = (const char*)p1;
+    g.ldw[0] = g.ldw[1] = ld;
+}
+void set_o(GemmArgs& g, int i, void* p, int64_t ld) {
+    g.o[i] = (char*)p;
+    g.ldo[i] = ld;
+}
+
+int ffn_forward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, char* ws) {
+    const rt_gated_ffn& a = f.a;
+    const int64_t es = f.es;
+    char* h = ws;
+    GemmArgs g;
+    memset(&g, 0, sizeof g);
+    g.part = (float*)(ws + f.h_bytes);
+    g.act = a.act;
+    g.alpha = a.alpha;
+    set_x(g, a.x, a.x, a.ldx * es);
+    set_w(g, a.w_gate, a.w_up, a.ld_in * es);
+    set_o(g, 0, h, f.ldh * es);
+    set_o(g, 1, a.pre_gate, a.ld_pre * es);
+    set_o(g, 2, a.pre_up, a.ld_pre * es);
+    int rc = run_product(ctx, v, a.dtype, f.gated, g);
+    if (rc) return rc;
+    set_x(g, h, h, f.ldh * es);
+    set_w(g, a.w_down, a.w_down, a.ld_down * es);
+    set_o(g, 0, a.out, a.ld_out * es);
+    return run_product(ctx, v, a.dtype, f.down, g);
+}
+
+int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_ffn_grads& r, char* ws) {
+    const rt_gated_ffn& a = f.a;
+    const int64_t es = f.es, ldh = f.ldh * es;
+    char *dg = ws, *du = ws + f.h_bytes, *h = ws + 2 * f.h_bytes;
+    GemmArgs g;
+    memset(&g, 0, sizeof g);
+    g.part = (float*)(ws + 3 * f.h_bytes);
+    g.act = a.act;
+    g.alpha = a.alpha;
+    int rc;
+    // dh = dout Wd^T, and from it what the gate's and up's sums get, and h again
+    set_x(g, r.dout, r.dout, r.ld_dout * es);
+    set_w(g, a.w_down, a.w_down, a.ld_down * es);
+    set_o(g, 0, dg, ldh);
+    set_o(g, 1, du, ldh);
+    set_o(g, 2, h, ldh);
+    g.e[0] = (const char*)a.pre_gate;
+    g.e[1] = (const char*)a.pre_up;
+    g.lde = a.ld_pre * es;
+    if ((rc = run_product(ctx, v, a.dtype, f.dh, g))) return rc;
+    if (r.dx) {                      // dx = dgate Wg^T + dup Wu^T: one sum over both
+        set_x(g, dg, du, ldh);
+        set_w(g, a.w_gate, a.w_up, a.ld_in * es);
+        set_o(g, 0, r.dx, r.ld_dx * es);
+        if ((rc = run_product(ctx, v, a.dtype, f.dx, g))) return rc;
+    }
+    if (r.dw_gate || r.dw_up) {      // x^T dgate and x^T dup side by side
+        Product p = f.dw_in;
+        set_x(g, a.x, a.x, a.ldx * es);
+        set_w(g, r.dw_gate ? dg : du, r.dw_up ? du : dg, ldh);
+        set_o(g, 0, r.dw_gate ? r.dw_gate : r.dw_up, r.ld_dw_in * es);
+        set_o(g, 1, r.dw_up, r.ld_dw_in * es);
+        p.nbatch = r.dw_gate && r.dw_up ? 2 : 1;
+        if ((rc = run_product(ctx, v, a.dtype, p, g))) return rc;
+    }
+    if (r.dw_down) {
+        set_x(g, h, h, ldh);
+        set_w(g, r.dout, r.dout, r.ld_dout * es);
+        set_o(g, 0, r.dw_down, r.ld_dw_down * es);
+        if ((rc = run_product(ctx, v, a.dtype, f.dw_down, g))) return rc;
+    }
+    return RT_OK;
+}
+
+// ---- the norms ----------------------------------------------------------------------------------------------------
+struct Norm {
+    rt_block_norm a;
+    int es;
+    int tpr;                         // threads of a row
+    int units;
+    int64_t rows_per_unit;
+    size_t part, ws;                 // bytes of one [units][d] array; of the workspace
+};
+
+int norm_make(rt_ctx* ctx, const char* fn, const rt_block_norm* in, int cus, Norm& m) {
+    if (!in) return failf(ctx, RT_EINVAL, "%s: the arguments are NULL", fn);
+    m.a = *in;
+    rt_block_norm& a = m.a;
+    if (a.dtype != RT_F32 && a.dtype != RT_BF16 && a.dtype != RT_F16) return failf(ctx, RT_EINVAL, "%s: unknown dtype %d", fn, a.dtype);
+    if (a.kind != RT_NORM_RMS && a.kind != RT_NORM_LAYER) return failf(ctx, RT_EINVAL, "%s: unknown kind of norm %d", fn, a.kind);
+    m.es = elem_size(a.dtype);
+    const int d_max = a.dtype == RT_F32 ? 16384 : 32768;
+    if (a.T < 0 || a.T > MAX_ROWS) return failf(ctx, RT_EINVAL, "%s: T = %lld", fn, (long long)a.T);
+    if (a.d < 1) return failf(ctx, RT_EINVAL, "%s: d = %d", fn, a.d);
+    if (a.d > d_max) return failf(ctx, RT_EUNSUPPORTED, "%s: d = %d: at most %d of this type fit a workgroup's registers", fn, a.d, d_max);
+    if (!(a.eps >= 0.0f) || !isfinite(a.eps) || !isfinite(a.res_scale) || !isfinite(a.branch_scale) || !isfinite(a.w_offset))
+        return failf(ctx, RT_EINVAL, "%s: eps must be >= 0, and it and the scales finite", fn);
+    if (a.gate && a.rows_per_gate < 1) return failf(ctx, RT_EINVAL, "%s: rows_per_gate = %lld", fn, (long long)a.rows_per_gate);
+    if (!a.gate || a.rows_per_gate > (a.T > 0 ? a.T : 1)) a.rows_per_gate = a.T > 0 ? a.T : 1;
+    if (!a.ldx) a.ldx = a.d;
+    if (!a.ld_branch) a.ld_branch = a.d;
+    if (!a.ldy) a.ldy = a.d;
+    if (!a.ldn) a.ldn = a.d;
+    if (!a.ld_gate) a.ld_gate = a.d;
+    if (a.T > 0x7fffffffll)
+        return failf(ctx, RT_EUNSUPPORTED, "%s: T = %lld rows are more than one launch covers", fn, (long long)a.T);
+    const int chunks = (a.d + 16 / m.es - 1) / (16 / m.es);
+    m.tpr = chunks <= 256 ? 64 : chunks <= 1024 ? 256 : 1024;
+    // units: enough to fill the chip, consecutive rows each; whole gate groups where a unit can hold some
+    const int64_t fill = (int64_t)cus * (m.tpr == 64 ? 16 : m.tpr == 256 ? 4 : 1);
+    int64_t r = (a.T + fill - 1) / fill;
+    if (r < 1) r = 1;
+    if (a.gate && a.rows_per_gate <= r) r = r / a.rows_per_gate * a.rows_per_gate;
+    m.rows_per_unit = r;
+    m.units = (int)((a.T + r - 1) / r);
+    m.part = (size_t)m.units * a.d * sizeof(float);
+    m.ws = m.part * 2 + (a.gate && a.rows_per_gate > r ? 2 * m.part : 0);
+    return RT_OK;
+}
+
+template <int DT, bool AL, int TPR, int NV>
+void launch_norm(hipStream_t st, const NormArgs& a, int what) {
+    constexpr int B = norm_block(TPR), RPB = B / TPR;
+    if (what == 0)
+        hipLaunchKernelGGL((norm_kernel<DT, TPR, NV, AL>), dim3((unsigned)((a.T + RPB - 1) / RPB)), dim3(B), 0, st, a);
+    else
+        hipLaunchKernelGGL((norm_back_kernel<DT, TPR, NV, AL>), dim3((unsigned)((a.units + RPB - 1) / RPB)), dim3(B), 0, st, a);
+}
+
+template <int DT, bool AL>
+void pick_norm(hipStream_t st, const NormArgs& a, int tpr, int what) {
+    const int nv = ((a.d + EPC<DT> - 1) / EPC<DT> + tpr - 1) / tpr;
+    if (tpr == 64) {
+        if (nv <= 1) launch_norm<DT, AL, 64, 1>(st, a, what);
+        else if (nv <= 2) launch_norm<DT, AL, 64, 2>(st, a, what);
+        else launch_norm<DT, AL, 64, 4>(st, a, what);
+    } else if (tpr == 256) {
+        if (nv <= 2) launch_norm<DT, AL, 256, 2>(st, a, what);
+        else launch_norm<DT, AL, 256, 4>(st, a, what);
+    } else {
+        if (nv <= 2) launch_norm<DT, AL, 1024, 2>(st, a, what);
+        else launch_norm<DT, AL, 1024, 4>(st, a, what);
+    }
+}
+
+int run_norm(rt_ctx* ctx, hipStream_t st, int dtype, const NormArgs& a, int tpr, int what, bool al) {
+    if (dtype == RT_F32) al ? pick_norm<RT_F32, true>(st, a, tpr, what) : pick_norm<RT_F32, false>(st, a, tpr, what);
+    else if (dtype == RT_BF16) al ? pick_norm<RT_BF16, true>(st, a, tpr, what) : pick_norm<RT_BF16, false>(st, a, tpr, what);
+    else al ? pick_norm<RT_F16, true>(st, a, tpr, what) : pick_norm<RT_F16, false>(st, a, tpr, what);
+    HIPCHK(ctx, hipGetLastError());
+    return RT_OK;
+}
+
+struct Aligned {                     // whether every row of every matrix starts on 16 bytes and ends on a whole chunk
+    bool ok = true;
+    int es;
+    void operator()(const void* p, int64_t ld, int64_t width) {
+        if (p) ok = ok && (uintptr_t)p % 16 == 0 && ld * es % 16 == 0 && width * es % 16 == 0;
+    }
+};
+
+void norm_args(const Norm& m, NormArgs& k) {
+    const rt_block_norm& a = m.a;
+    const int64_t es = m.es;
+    memset(&k, 0, sizeof k);
+    k.T = a.T; k.d = a.d; k.kind = a.kind;
+    k.eps = a.eps; k.rs = a.res_scale; k.bs = a.branch_scale; k.w_off = a.w_offset; k.rpg = a.rows_per_gate;
+    k.x = (const char*)a.x; k.b = (const char*)a.branch; k.gate = (const char*)a.gate;
+    k.w_post = (const char*)a.w_post; k.w_pre = (const char*)a.w_pre;
+    k.y = (char*)a.y; k.n = (char*)a.n;
+    k.ldx = a.ldx * es; k.ldb = a.ld_branch * es; k.ldy = a.ldy * es; k.ldn = a.ldn * es; k.ldg = a.ld_gate * es;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rt_ctx_stream(rt_ctx* ctx, void** stream) {
+    if (!ctx) return RT_EINVAL;
+    if (!stream) return failf(ctx, RT_EINVAL, "rt_ctx_stream: stream is NULL");
+    RtCtxView v;
+    rt_ctx_view(ctx, &v);
+    *stream = (void*)v.stream;
+    return RT_OK;
+}
+
+int rt_gated_ffn_workspace(rt_ctx* ctx, const rt_gated_ffn* a, int backward, size_t* bytes) {
+    if (!ctx) return RT_EINVAL;
+    if (!bytes) return failf(ctx, RT_EINVAL, "rt_gated_ffn_workspace: bytes is NULL");
+    RtCtxView v;
+    rt_ctx_view(ctx, &v);
+    Ffn f;
+    const int rc = ffn_make(ctx, "rt_gated_ffn_workspace", a, v.cu_count, f);
+    if (rc) return rc;
+    *bytes = backward ? f.ws_bwd : f.ws_fwd;
+    return RT_OK;
+}
+
+int rt_gated_ffn_dev(rt_ctx* ctx, const rt_gated_ffn* args, void* ws, size_t ws_bytes) {
+    static const char fn[] = "rt_gated_ffn_dev";
+    if (!ctx) return RT_EINVAL;
+    RtCtxView v;
+    rt_ctx_view(ctx, &v);
+    Ffn f;
+    int rc = ffn_make(ctx, fn, args, v.cu_count, f);
+    if (rc) return rc;
+    const rt_gated_ffn& a = f.a;
+    const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in},
+                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down}};
+    const Mat out[] = {{"out", a.out, a.T, a.d_out, a.ld_out}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre},
+                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre}, {"the workspace", ws, 1, (int64_t)(f.ws_fwd / f.es), (int64_t)(f.ws_fwd / f.es)}};
+    for (const Mat& m : in)
+        if ((rc = check_mat(ctx, fn, m, f.es, true))) return rc;
+    for (int i = 0; i < 3; ++i)
+        if ((rc = check_mat(ctx, fn, out[i], f.es, i == 0))) return rc;
+    if (!a.pre_gate != !a.pre_up) return failf(ctx, RT_EINVAL, "%s: give both of pre_gate and pre_up, or neither", fn);
+    if (a.T == 0) return RT_OK;
+    if ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_fwd)) || (rc = check_disjoint(ctx, fn, in, 4, out, 4, f.es))) return rc;
+    DeviceScope dev(v.device);
+    HIPCHK(ctx, dev.err);
+    return ffn_forward(ctx, v, f, (char*)ws);
+}
+
+int rt_gated_ffn_backward_dev(rt_ctx* ctx, const rt_gated_ffn* args, const rt_gated_ffn_grads* grads, void* ws, size_t ws_bytes) {
+    static const char fn[] = "rt_gated_ffn_backward_dev";
+    if (!ctx) return RT_EINVAL;
+    if (!grads) return failf(ctx, RT_EINVAL, "%s: the gradients are NULL", fn);
+    RtCtxView v;
+    rt_ctx_view(ctx, &v);
+    Ffn f;
+    int rc = ffn_make(ctx, fn, args, v.cu_count, f);
+    if (rc) return rc;
+    const rt_gated_ffn& a = f.a;
+    rt_gated_ffn_grads r = *grads;
+    if (!r.ld_dout) r.ld_dout = a.d_out;
+    if (!r.ld_dx) r.ld_dx = a.d_in;
+    if (!r.ld_dw_in) r.ld_dw_in = a.d_ff;
+    if (!r.ld_dw_down) r.ld_dw_down = a.d_out;
+    const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in},
+                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre},
+                      {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre}, {"dout", r.dout, a.T, a.d_out, r.ld_dout}};
+    const Mat out[] = {{"dx", r.dx, a.T, a.d_in, r.ld_dx}, {"dw_gate", r.dw_gate, a.d_in, a.d_ff, r.ld_dw_in},
+                       {"dw_up", r.dw_up, a.d_in, a.d_ff, r.ld_dw_in}, {"dw_down", r.dw_down, a.d_ff, a.d_out, r.ld_dw_down},
+                       {"the workspace", ws, 1, (int64_t)(f.ws_bwd / f.es), (int64_t)(f.ws_bwd / f.es)}};
+    for (const Mat& m : in)
+        if ((rc = check_mat(ctx, fn, m, f.es, true))) return rc;
+    for (int i = 0; i < 4; ++i)
+        if ((rc = check_mat(ctx, fn, out[i], f.es, false))) return rc;
+    if (a.T > 0 && ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_bwd)))) return rc;
+    if ((rc = check_disjoint(ctx, fn, in, 7, out, a.T > 0 ? 5 : 4, f.es))) return rc;
+    DeviceScope dev(v.device);
+    HIPCHK(ctx, dev.err);
+    if (a.T == 0) {
+        if ((rc = zero_rows(ctx, v.stream, r.dw_gate, r.ld_dw_in * f.es, a.d_in, (int64_t)a.d_ff * f.es)) ||
+            (rc = zero_rows(ctx, v.stream, r.dw_up, r.ld_dw_in * f.es, a.d_in, (int64_t)a.d_ff * f.es)))
+            return rc;
+        return zero_rows(ctx, v.stream, r.dw_down, r.ld_dw_down * f.es, a.d_ff, (int64_t)a.d_out * f.es);
+    }
+    return ffn_backward(ctx, v, f, r, (char*)ws);
+}
+
+int rt_block_norm_workspace(rt_ctx* ctx, const rt_block_norm* a, size_t* bytes) {
+    if (!ctx) return RT_EINVAL;
+    if (!bytes) return failf(ctx, RT_EINVAL, "rt_block_norm_workspace: bytes is NULL");
+    RtCtxView v;
+    rt_ctx_view(ctx, &v);
+    Norm m;
+    const int rc = norm_make(ctx, "rt_block_norm_workspace", a, v.cu_count, m);
+    if (rc) return rc;
+    *bytes = m.ws;
+    return RT_OK;
+}
+
+int rt_block_norm_dev(rt_ctx* ctx, const rt_block_norm* args) {
+    static const char fn[] = "rt_block_norm_dev";
+    if (!ctx) return RT_EINVAL;
+    RtCtxView v;
+    rt_ctx_view(ctx, &v);
+    Norm m;
+    int rc = norm_make(ctx, fn, args, v.cu_count, m);
+    if (rc) return rc;
+    const rt_block_norm& a = m.a;
+    const int64_t gates = (a.T + a.rows_per_gate - 1) / a.rows_per_gate;
+    const Mat in[] = {{"x", a.x, a.T, a.d, a.ldx}, {"branch", a.branch, a.T, a.d, a.ld_branch}, {"gate", a.gate, gates, a.d, a.ld_gate},
+                      {"w_post", a.w_post, 1, a.d, a.d}, {"w_pre", a.w_pre, 1, a.d, a.d}};
+    const Mat out[] = {{"y", a.y, a.T, a.d, a.ldy}, {"n", a.n, a.T, a.d, a.ldn}};
+    for (int i = 0; i < 5; ++i)
+        if ((rc = check_mat(ctx, fn, in[i], m.es, i == 0))) return rc;
+    for (const Mat& o : out)
+        if ((rc = check_mat(ctx, fn, o, m.es, false))) return rc;
+    if (a.gate && !a.branch) return failf(ctx, RT_EINVAL, "%s: a gate without a branch", fn);
+    if (a.T == 0) return RT_OK;
+    if (!a.y && !a.n) return failf(ctx, RT_EINVAL, "%s: y and n are both NULL", fn);
+    // rows are read before they are written: an output may take the place of x or of branch, whole
+    for (const Mat& o : out)
+        for (int i = 0; i < 5; ++i)
+            if (overlap(o, in[i], m.es) && !(i < 2 && same_place(o, in[i])))
+                return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, o.name, in[i].name);
+    if (overlap(out[0], out[1], m.es)) return failf(ctx, RT_EINVAL, "%s: y and n overlap", fn);
+    DeviceScope dev(v.device);
+    HIPCHK(ctx, dev.err);
+    NormArgs k;
+    norm_args(m, k);
+    Aligned al;
+    al.es = m.es;
+    for (const Mat& x : in) al(x.p, x.ld, x.width);
+    for (const Mat& x : out) al(x.p, x.ld, x.width);
+    return run_norm(ctx, v.stream, a.dtype, k, m.tpr, 0, al.ok);
+}
+
+int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_block_norm_grads* grads, void* ws, size_t ws_bytes) {
+    static const char fn[] = "rt_block_norm_backward_dev";
+    if (!ctx) return RT_EINVAL;
+    if (!grads) return failf(ctx, RT_EINVAL, "%s: the gradients are NULL", fn);
+    RtCtxView v;
+    rt_ctx_view(ctx, &v);
+    Norm m;
+    int rc = norm_make(ctx, fn, args, v.cu_count, m);
+    if (rc) return rc;
+    const rt_block_norm& a = m.a;
+    rt_block_norm_grads r = *grads;
+    if (!r.ld_dy) r.ld_dy = a.d;
+    if (!r.ld_dn) r.ld_dn = a.d;
+    if (!r.ld_dx) r.ld_dx = a.d;
+    if (!r.ld_dbranch) r.ld_dbranch = a.d;
+    if (!r.ld_dgate) r.ld_dgate = a.d;
+    const int64_t gates = (a.T + a.rows_per_gate - 1) / a.rows_per_gate;
+    // without a branch y is res_scale * x, and x stands in for a y that was not written
+    const bool from_x = !a.y && !a.branch;
+    const Mat yin = from_x ? Mat{"x", a.x, a.T, a.d, a.ldx} : Mat{"y", a.y, a.T, a.d, a.ldy};
+    const Mat in[] = {yin, {"branch", a.branch, a.T, a.d, a.ld_branch}, {"dy", r.dy, a.T, a.d, r.ld_dy}, {"dn", r.dn, a.T, a.d, r.ld_dn},
+                      {"gate", a.gate, gates, a.d, a.ld_gate}, {"w_post", a.w_post, 1, a.d, a.d}, {"w_pre", a.w_pre, 1, a.d, a.d}};
+    const Mat out[] = {{"dx", r.dx, a.T, a.d, r.ld_dx}, {"dbranch", r.dbranch, a.T, a.d, r.ld_dbranch}, {"dgate", r.dgate, gates, a.d, r.ld_dgate},
+                       {"dw_post", r.dw_post, 1, a.d, a.d}, {"dw_pre", r.dw_pre, 1, a.d, a.d},
+                       {"the workspace", ws, 1, (int64_t)(m.ws / m.es), (int64_t)(m.ws / m.es)}};
+    for (int i = 0; i < 7; ++i)
+        if ((rc = check_mat(ctx, fn, in[i], m.es, i == 0 && r.dn))) return rc;
+    for (int i = 0; i < 5; ++i)
+        if ((rc = check_mat(ctx, fn, out[i], m.es, false))) return rc;
+    if (a.T > 0 && !r.dy && !r.dn) return failf(ctx, RT_EINVAL, "%s: dy and dn are both NULL", fn);
+    if (a.gate && !a.branch) return failf(ctx, RT_EINVAL, "%s: a gate without a branch", fn);
+    if (!a.branch && (r.dbranch || r.dgate || r.dw_post)) return failf(ctx, RT_EINVAL, "%s: dbranch, dgate or dw_post without a branch", fn);
+    if (!a.gate && r.dgate) return failf(ctx, RT_EINVAL, "%s: dgate without a gate", fn);
+    if (a.T > 0 && (rc = check_ws(ctx, fn, ws, ws_bytes, m.ws))) return rc;
+    // a row's dx is written when its y, dy and dn have been read, its dbranch when all of it has
+    for (int i = 0; i < (a.T > 0 ? 6 : 5); ++i) {
+        for (int j = 0; j < 7; ++j) {
+            const bool fine = same_place(out[i], in[j]) && ((i == 0 && (j == 0 || j == 2 || j == 3)) || (i == 1 && j < 4));
+            if (overlap(out[i], in[j], m.es) && !fine) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, in[j].name);
+        }
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j], m.es)) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, out[j].name);
+    }
+    DeviceScope dev(v.device);
+    HIPCHK(ctx, dev.err);
+    if (a.T == 0) {
+        if ((rc = zero_rows(ctx, v.stream, r.dw_post, (int64_t)a.d * m.es, 1, (int64_t)a.d * m.es))) return rc;
+        return zero_rows(ctx, v.stream, r.dw_pre, (int64_t)a.d * m.es, 1, (int64_t)a.d * m.es);
+    }
+    NormArgs k;
+    norm_args(m, k);
+    const int64_t es = m.es;
+    k.yin = (const char*)yin.p; k.ldy = yin.ld * es; k.yin_scale = from_x ? a.res_scale : 1.0f;
+    k.dy = (const char*)r.dy; k.dn = (const char*)r.dn;
+    k.dx = (char*)r.dx; k.db = (char*)r.dbranch; k.dgate = (char*)r.dgate;
+    k.lddy = r.ld_dy * es; k.lddn = r.ld_dn * es; k.lddx = r.ld_dx * es; k.lddb = r.ld_dbranch * es; k.lddg = r.ld_dgate * es;
+    k.want_post = r.dw_post != nullptr; k.want_pre = r.dw_pre != nullptr && r.dn != nullptr;
+    k.rows_per_unit = m.rows_per_unit; k.units = m.units;
+    k.p_post = (float*)ws; k.p_pre = (float*)((char*)ws + m.part); k.p_gate = (float*)((char*)ws + 2 * m.part);
+    k.dw_post = (char*)r.dw_post; k.dw_pre = k.want_pre ? (char*)r.dw_pre : nullptr;
+    Aligned al;
+    al.es = m.es;
+    for (const Mat& x : in) al(x.p, x.ld, x.width);
+    for (int i = 0; i < 5; ++i) al(out[i].p, out[i].ld, out[i].width);
+    if ((rc = run_norm(ctx, v.stream, a.dtype, k, m.tpr, 1, al.ok))) return rc;
+    if (r.dw_pre && !r.dn && (rc = zero_rows(ctx, v.stream, r.dw_pre, (int64_t)a.d * es, 1, (int64_t)a.d * es))) return rc;
+    // what is left to join: the weights' sums, and the gates that more than one unit saw
+    const bool gates_left = r.dgate && a.rows_per_gate > m.rows_per_unit;
+    const int first = k.want_post || k.want_pre ? 0 : 2, last = gates_left ? 2 + (int)gates : 2;
+    if (last > first) {
+        const dim3 grid((a.d + 31) / 32, last - first);
+        if (a.dtype == RT_F32) hipLaunchKernelGGL(norm_join_kernel<RT_F32>, grid, dim3(256), 0, v.stream, k, first);
+        else if (a.dtype == RT_BF16) hipLaunchKernelGGL(norm_join_kernel<RT_BF16>, grid, dim3(256), 0, v.stream, k, first);
+        else hipLaunchKernelGGL(norm_join_kernel<RT_F16>, grid, dim3(256), 0, v.stream, k, first);
+        HIPCHK(ctx, hipGetLastError());
+    }
+    return RT_OK;
+}
+
+}  // extern "C"

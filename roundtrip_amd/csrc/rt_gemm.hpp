@@ -1,0 +1,383 @@
+// rt_gemm.hpp — the matrix products of the gated feed-forward block, on the matrix cores, with their epilogues.
+//
+//   C[m][n] = sum over k of X[m][k] W[k][n]           X: rows (tokens, or the rows of a weight gradient), W: columns
+//
+// Each operand lies in memory with k contiguous (LK) or with its own index contiguous (LI): weights are [in, out], so the
+// forward products read W as LI, the products with a transposed weight as LK, and a weight gradient (k = tokens) reads
+// both as LI.  Tiles of 128 bytes of k go through LDS, two in turn; the matrix instruction is 16x16x32 (16-bit types) or
+// 16x16x4 (float32) with W as its rows and X as its columns, so that a lane holds four neighbouring n of one m.
+#pragma once
+#include "rt_elem.hpp"
+
+enum { LK = 0, LI = 1 };
+enum { EPI_STORE = 0, EPI_GATED = 1, EPI_GATED_BWD = 2 };
+
+struct GemmArgs {
+    const char* x[2];              // two K segments (nseg = 2), or one operand for each blockIdx.z
+    const char* w[2];              // ... EPI_GATED: gate and up
+    long long ldx[2], ldw[2];      // bytes
+    long long M, K;
+    int N;
+    int nseg;                      // K segments: C = x[0] w[0] + x[1] w[1]
+    int nk;                        // K tiles of a segment
+    int tiles_m, tiles_n;
+    int splits, per_split;         // K tiles are dealt to blockIdx.y, per_split each
+    float* part;                   // splits > 1: [split][slot][M][Np] partial sums, joined by gemm_join_kernel
+    int Np, nslot;
+    char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two may be NULL).
+    long long ldo[3];              // EPI_GATED_BWD: dgate, dup, h
+    const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept
+    long long lde;
+    int act;
+    float alpha;
+};
+
+// ---- the gate's activation ----------------------------------------------------------------------------------------
+// s(t) = 1 / (1 + exp(-t)).  16-bit results: hardware exp2 and reciprocal (each <= 1 ulp of float32, far below the
+// rounding of the result).
+template <int DT>
+__device__ __forceinline__ float sigmoid_f(float t) {
+    if (ES<DT> == 4) return 1.0f / (1.0f + expf(-t));
+    return __builtin_amdgcn_rcpf(1.0f + __expf(-t));
+}
+
+// a = act(g), d = act'(g).  gelu: the tanh form, 0.5 g (1 + tanh z) = g s(2z), which loses nothing where tanh z is near -1.
+template <int DT>
+__device__ __forceinline__ void act_f(int act, float alpha, float g, float& a, float& d) {
+    if (act == RT_ACT_LRELU) {
+        d = g > 0.0f ? 1.0f : alpha;
+        a = g * d;
+        return;
+    }
+    if (act == RT_ACT_GELU_TANH) {
+        const float c2 = 1.5957691216057308f, c3 = 0.044715f;      // 2 sqrt(2 / pi)
+        const float s = sigmoid_f<DT>(c2 * (g + c3 * g * g * g));
+        a = g * s;
+        d = s + a * (1.0f - s) * c2 * (1.0f + 3.0f * c3 * g * g);
+        return;
+    }
+    const float s = sigmoid_f<DT>(g);
+    a = act == RT_ACT_SILU ? g * s : s;
+    d = act == RT_ACT_SILU ? s * (1.0f + g * (1.0f - s)) : s * (1.0f - s);
+}
+
+// What becomes of four neighbouring sums of row m, columns n .. n+3 (v1: the second of EPI_GATED).
+template <int DT, int EPI>
+__device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, int n, f32x4 v0, f32x4 v1) {
+    const int valid = a.N - n;
+    if (valid <= 0) return;
+    const long long c = (long long)n * ES<DT>;
+    if (EPI == EPI_STORE) {
+        store4<DT>(a.o[z] + m * a.ldo[z] + c, v0, valid);
+    } else if (EPI == EPI_GATED) {
+        f32x4 h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float t, d;
+            act_f<DT>(a.act, a.alpha, v0[j], t, d);
+            h[j] = t * v1[j];
+        }
+        store4<DT>(a.o[0] + m * a.ldo[0] + c, h, valid);
+        if (a.o[1]) {
+            store4<DT>(a.o[1] + m * a.ldo[1] + c, v0, valid);
+            store4<DT>(a.o[2] + m * a.ldo[2] + c, v1, valid);
+        }
+    } else {
+        const f32x4 g = load4<DT>(a.e[0] + m * a.lde + c, valid), u = load4<DT>(a.e[1] + m * a.lde + c, valid);
+        f32x4 dg, du, h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float t, d;
+            act_f<DT>(a.act, a.alpha, g[j], t, d);
+            dg[j] = v0[j] * u[j] * d;
+            du[j] = v0[j] * t;
+            h[j] = t * u[j];
+        }
+        store4<DT>(a.o[0] + m * a.ldo[0] + c, dg, valid);
+        store4<DT>(a.o[1] + m * a.ldo[1] + c, du, valid);
+        store4<DT>(a.o[2] + m * a.ldo[2] + c, h, valid);
+    }
+}
+
+// ---- tiles --------------------------------------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int OOB = 0x7fffff00;            // an offset that every buffer below ends before
+
+// One operand's tile in LDS: R of its rows (or columns) x 128 bytes of k, as 16-byte chunks.
+//   LK: [row][8 chunks], chunk c of row r at c ^ ((r >> 1) & 7): sixteen rows' reads of one chunk fall into sixteen
+//       different 16-byte slots of the 256 bytes that LDS serves at once.
+//   LI: [k][row], NSUB sub-tiles of R / NSUB rows one behind the other.  16-bit types are read with ds_read_b64_tr_b16
+//       (sixteen lanes read a 4 x 16 block, each gets a column): its 32-byte units are xored with (k & 3) | (k >> 3 & 1) << 2
+//       (rows of 128 bytes, two of which lie in those 256: (k >> 1 & 1) | (k >> 3 & 1) << 1); float32 is read four bytes a
+//       lane, 64 a row: its 64-byte units are xored with (k >> 2) & 3.
+template <int DT, int L, int R, int NSUB, int NT>
+struct Tile {
+    static constexpr int KE = 128 / ES<DT>;                 // k's of a tile
+    static constexpr int BYTES = R * 128;
+    static constexpr int SR = R / NSUB;
+    static constexpr int PITCH = L == LK ? 128 : SR * ES<DT>;
+    static constexpr int PC = PITCH / 16;
+    static constexpr int ITER = BYTES / 16 / NT;            // chunks a thread brings
+    static constexpr int SUB_CHUNKS = KE * PC;              // LI: chunks of a sub-tile
+    static_assert(BYTES % (16 * NT) == 0, "every thread brings whole chunks");
+    static_assert(L == LK ? NSUB == 1 : SR >= 64, "the xor needs that many units");
+
+    static __device__ __forceinline__ int unit_xor(int k) {       // LI, 16-bit types
+        return SR == 64 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : (k & 3) | (k >> 3 & 1) << 2;
+    }
+
+    // chunk it of thread tid: which row / k (idx), which chunk of it (c), which sub-tile
+    static __device__ __forceinline__ void place(int tid, int it, int& sub, int& idx, int& c) {
+        const int q = it * NT + tid;
+        if (L == LK) {
+            sub = 0;
+            idx = q >> 3;
+            c = (q & 7) ^ ((idx >> 1) & 7);
+        } else {
+            sub = q / SUB_CHUNKS;
+            const int p = q % PC;
+            idx = (q % SUB_CHUNKS) / PC;
+            c = ES<DT> == 4 ? ((((p >> 2) ^ ((idx >> 2) & 3)) << 2) | (p & 3))
+                            : ((((p >> 1) ^ unit_xor(idx)) << 1) | (p & 1));
+        }
+    }
+};
+
+template <int DT, int L, int R, int NSUB, int NT, bool AL>
+struct Loader {
+    typedef Tile<DT, L, R, NSUB, NT> T;
+    int voff[T::ITER];                // AL: byte offset from the tile's start; OOB where the row or column does not exist
+    u32x4 reg[AL ? 1 : T::ITER];      // !AL: chunks on their way through registers
+
+    // rows: how many of the tile's rows (LI: columns) exist, counted in a sub-tile
+    __device__ __forceinline__ void init(int tid, long long ld, int rows) {
+        if (!AL) return;
+#pragma unroll
+        for (int it = 0; it < T::ITER; ++it) {
+            int sub, idx, c;
+            T::place(tid, it, sub, idx, c);
+            const int row = L == LK ? idx : c * EPC<DT>;
+            voff[it] = row < rows ? (int)(idx * ld) + c * 16 : OOB;
+        }
+    }
+
+    // Brings the tile that starts at element k0 of K.  base: the operand's first row (LK) or column (LI) of this tile,
+    // base2: the second sub-tile's.
+    __device__ __forceinline__ void fetch(char* sm, const char* base, const char* base2, long long ld, long long k0, long long K,
+                                          int rows, int tid) {
+        const long long left = K - k0;
+        const int ke = left < T::KE ? (int)left : T::KE;
+        const long long adv = L == LK ? k0 * ES<DT> : k0 * ld;
+        if (AL) {
+            // a tile spans less than 2^31 bytes (the host bounds ld), whatever the whole operand spans
+            const int span = L == LK ? (int)((rows - 1) * ld) + ke * ES<DT> : (int)((ke - 1) * ld) + rows * ES<DT>;
+            const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+#pragma unroll
+            for (int it = 0; it < T::ITER; ++it) {
+                const bool second = L == LI && NSUB == 2 && it >= T::ITER / 2;
+                auto r = __builtin_amdgcn_make_buffer_rsrc((void*)((second ? base2 : base) + adv), 0, span, 0x00020000);
+                int v = voff[it];
+                if (L == LK && ke < T::KE) {            // the last tile: chunks behind K are zeros
+                    int sub, idx, c;
+                    T::place(tid, it, sub, idx, c);
+                    if (c * EPC<DT> >= ke) v = OOB;
+                }
+                if (L == LI && ke < T::KE) {            // k's behind K: behind the span, or before it ends in a short last row
+                    int sub, idx, c;
+                    T::place(tid, it, sub, idx, c);
+                    if (idx >= ke) v = OOB;
+                }
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(sm + (it * NT + wave * 64) * 16), 16, v, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int it = 0; it < T::ITER; ++it) {
+                int sub, idx, c;
+                T::place(tid, it, sub, idx, c);
+                const char* b = (L == LI && NSUB == 2 && sub ? base2 : base) + adv;
+                const int have = L == LK ? (idx < rows ? ke - c * EPC<DT> : 0) : (idx < ke ? rows - c * EPC<DT> : 0);
+                u32x4 r = {0, 0, 0, 0};
+                if (have > 0) r = load_chunk<DT, false>(b + idx * ld + c * 16, have);
+                reg[it] = r;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void land(char* sm, int tid) {
+        if (AL) return;
+#pragma unroll
+        for (int it = 0; it < T::ITER; ++it) *(u32x4*)(sm + (it * NT + tid) * 16) = reg[it];
+    }
+};
+
+// Reads the fragment of sixteen rows (or columns) starting at 16 t, k step s (of two): lane (g = lane / 16, i = lane % 16)
+// gets row i, k = 32 s + 8 g .. + 7 (16-bit), 16 s + 4 g .. + 3 (float32).  The same k's for both operands is all that
+// the sum needs.
+template <int DT, int L, int R, int NSUB, int NT>
+__device__ __forceinline__ u32x4 read_frag(const char* sm, int lane, int t, int s) {
+    typedef Tile<DT, L, R, NSUB, NT> T;
+    const int i = lane & 15, g = lane >> 4;
+    if (L == LK) {
+        return *(const u32x4*)(sm + (16 * t + i) * 128 + (((4 * s + g) ^ (i >> 1)) << 4));
+    } else {
+        constexpr int TS = T::SR / 16;                        // fragments of a sub-tile
+        sm += (t / TS) * (T::SUB_CHUNKS * 16);
+        t %= TS;
+        if (ES<DT> == 4) {
+            u32x4 r;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = *(const unsigned*)(sm + (16 * s + 4 * g + j) * T::PITCH + ((t ^ g) << 6) + i * 4);
+            return r;
+        }
+        union { s16x4 h[2]; u32x4 v; } u;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4*)(sm + (32 * s + 8 * g + 4 * h + (i >> 2)) * T::PITCH + ((t ^ T::unit_xor(8 * g + (i >> 2))) << 5) + (i & 3) * 8));
+        return u.v;
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma_step(u32x4 w, u32x4 x, f32x4 c) {
+    if constexpr (DT == RT_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), c, 0, 0, 0);
+    else if constexpr (DT == RT_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x), c, 0, 0, 0);
+    else {
+        const f32x4 wf = __builtin_bit_cast(f32x4, w), xf = __builtin_bit_cast(f32x4, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[j], xf[j], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// Workgroup -> tile.  Workgroups go to the eight XCDs in turn: each XCD gets a run of tiles, walked in bands of GM tile rows,
+// so that the tiles it works on at a time share their operands in its L2.
+__device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int n = tiles_m * tiles_n, q = n >> 3, r = n & 7, xcd = b & 7;
+    const int id = xcd * q + (xcd < r ? xcd : r) + (b >> 3);
+    constexpr int GM = 8;
+    const int band = id / (GM * tiles_n), first = band * GM;
+    const int h = tiles_m - first < GM ? tiles_m - first : GM;
+    const int in = id - band * GM * tiles_n;
+    tm = first + in % h;
+    tn = in / h;
+}
+
+// BM x BN sums a workgroup of WM x WN waves.  EPI_GATED: the BN columns are BN / 2 of the gate's and the same of up's, and
+// every wave holds both of its columns, so the product needs no exchange.
+template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool AL>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
+    constexpr int NT = 64 * WM * WN, DUAL = EPI == EPI_GATED ? 2 : 1;
+    typedef Tile<DT, LX, BM, 1, NT> TX;
+    typedef Tile<DT, LW, BN, DUAL, NT> TW;
+    constexpr int MT = BM / WM / 16, NTL = BN / WN / 16, CN = BN / DUAL;      // CN: columns of C a tile covers
+    __shared__ __attribute__((aligned(1024))) char sx0[TX::BYTES], sw0[TW::BYTES], sx1[TX::BYTES], sw1[TW::BYTES];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN, z = blockIdx.z, split = blockIdx.y;
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const long long m0 = (long long)tm * BM;
+    const int n0 = tn * CN;
+    const int mrows = a.M - m0 < BM ? (int)(a.M - m0) : BM, nrows = a.N - n0 < CN ? a.N - n0 : CN;
+    const int t0 = split * a.per_split, t_all = a.nk * a.nseg, t1 = t0 + a.per_split < t_all ? t0 + a.per_split : t_all;
+
+    Loader<DT, LX, BM, 1, NT, AL> lx;
+    Loader<DT, LW, BN, DUAL, NT, AL> lw;
+    lx.init(tid, a.ldx[0], mrows);
+    lw.init(tid, a.ldw[0], nrows);
+    f32x4 acc[MT][NTL];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+    auto fetch = [&](char* sx, char* sw, int t) __attribute__((always_inline)) {
+        const int seg = t >= a.nk ? 1 : 0;
+        const long long k0 = (long long)(t - (seg ? a.nk : 0)) * TX::KE;
+        const int ix = seg | z, iw = EPI == EPI_GATED ? 0 : (seg | z);
+        const char* bx = a.x[ix] + (LX == LK ? m0 * a.ldx[0] : m0 * ES<DT>);
+        const long long nw = LW == LK ? n0 * a.ldw[0] : (long long)n0 * ES<DT>;
+        lx.fetch(sx, bx, nullptr, a.ldx[0], k0, a.K, mrows, tid);
+        lw.fetch(sw, a.w[iw] + nw, EPI == EPI_GATED ? a.w[1] + nw : nullptr, a.ldw[0], k0, a.K, nrows, tid);
+    };
+    auto land = [&](char* sx, char* sw) __attribute__((always_inline)) {
+        lx.land(sx, tid);
+        lw.land(sw, tid);
+        __builtin_amdgcn_s_waitcnt(0x0f70);          // vmcnt(0): the chunks on their way to LDS have arrived
+        __syncthreads();
+    };
+    auto compute = [&](const char* sx, const char* sw) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 fx[MT], fw[NTL];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fx[i] = read_frag<DT, LX, BM, 1, NT>(sx, lane, wm * MT + i, s);
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) {
+                constexpr int H = NTL / DUAL;
+                const int t = DUAL == 2 ? (j / H) * (CN / 16) + wn * H + j % H : wn * NTL + j;
+                fw[j] = read_frag<DT, LW, BN, DUAL, NT>(sw, lane, t, s);
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) acc[i][j] = mfma_step<DT>(fw[j], fx[i], acc[i][j]);
+        }
+    };
+
+    fetch(sx0, sw0, t0);
+    land(sx0, sw0);
+    for (int t = t0; t < t1; t += 2) {
+        if (t + 1 < t1) fetch(sx1, sw1, t + 1);
+        compute(sx0, sw0);
+        if (t + 1 >= t1) break;
+        land(sx1, sw1);
+        if (t + 2 < t1) fetch(sx0, sw0, t + 2);
+        compute(sx1, sw1);
+        if (t + 2 < t1) land(sx0, sw0);
+    }
+
+    const int i = lane & 15, g = lane >> 4;
+    constexpr int H = NTL / DUAL;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const long long m = m0 + wm * (BM / WM) + mt * 16 + i;
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            const int n = n0 + wn * (CN / WN) + j * 16 + 4 * g;
+            if (a.splits > 1) {
+                if (n < a.Np) {
+#pragma unroll
+                    for (int d = 0; d < DUAL; ++d)
+                        *(f32x4*)(a.part + (((long long)split * a.nslot + (DUAL == 2 ? d : z)) * a.M + m) * a.Np + n) = acc[mt][j + d * H];
+                }
+            } else {
+                epilogue<DT, EPI>(a, z, m, n, acc[mt][j], acc[mt][DUAL == 2 ? j + H : j]);
+            }
+        }
+    }
+}
+
+// Joins the partial sums of the K splits, in their order, and finishes them.
+template <int DT, int EPI>
+__global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
+    const int quads = a.Np >> 2, z = blockIdx.z;
+    const long long total = a.M * quads, slot = a.M * a.Np;
+    for (long long p = (long long)blockIdx.x * 256 + threadIdx.x; p < total; p += (long long)gridDim.x * 256) {
+        const long long m = p / quads;
+        const int n = (int)(p - m * quads) * 4;
+        const float* q = a.part + (long long)z * slot + m * a.Np + n;
+        f32x4 v0 = {0, 0, 0, 0}, v1 = {0, 0, 0, 0};
+        for (int s = 0; s < a.splits; ++s) {
+            v0 += *(const f32x4*)(q + (long long)s * a.nslot * slot);
+            if (EPI == EPI_GATED) v1 += *(const f32x4*)(q + ((long long)s * a.nslot + 1) * slot);
+        }
+        epilogue<DT, EPI>(a, z, m, n, v0, v1);
+    }
+}

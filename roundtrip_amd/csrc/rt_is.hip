@@ -32,7 +32,7 @@
 #include <dlfcn.h>
 #include <rccl/rccl.h>      // types and prototypes only: librccl.so.1 (573 MB) is dlopen'ed by rt_comm_init, never linked
 
-#include "../../include/rt_is.h"
+#include "rt_internal.hpp"
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -642,6 +642,14 @@ int mean_stderr_enqueue(rt_ctx* ctx, const double* v, int64_t N, double* out2) {
 }
 
 }  // namespace
+
+void rt_ctx_view(const rt_ctx* ctx, RtCtxView* out) {
+    out->device = ctx->device;
+    out->cu_count = ctx->cu_count;
+    out->stream = ctx->stream;
+}
+
+int rt_ctx_fail(rt_ctx* ctx, int code, const char* msg) { return fail(ctx, code, msg); }
 
 extern "C" {
 
