@@ -151,7 +151,7 @@ def prepare(case, seed):
         act = {"silu": eng.SILU, "gelu": eng.GELU_TANH, "lrelu": eng.LRELU, "sigmoid": eng.SIGMOID}[case["act"]]
         x = s["x"] if case["op"] == "ffn" else new(T, d)
         b = new(T, d)
-        s["pre"] = (new(T, f), new(T, f)) if train else (None, None)
+        s["pre"] = [torch.empty((T, f), device="cuda") if train else None for _ in range(2)]       # float32 in every type
         s["ffn"] = eng.gated_ffn_args(T, d, f, d, code, act, x=p(x), w_gate=p(s["w_gate"]), w_up=p(s["w_up"]),
                                       w_down=p(s["w_down"]), out=p(b), pre_gate=p(s["pre"][0]), pre_up=p(s["pre"][1]),
                                       alpha=ALPHA)
