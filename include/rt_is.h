@@ -280,7 +280,7 @@ uint32_t rt_crc32c(const void* data, size_t n, uint32_t crc);
  * The layers deep networks put around and between plain dense ones, next to rt_mlp_forward_dev: a gated feed-forward block
  * and the norms before and after it, forward and backward.  NO COUNTERPART IN THE REFERENCE (its networks are chains of
  * dense layers, model.py:61-88).
- *   - all pointers in the structs are DEVICE pointers to arrays of the call's dtype, rows contiguous; an ld* is the distance
+ *   - all pointers in the structs are DEVICE pointers to arrays of the call's dtype (but for pre_gate, pre_up), rows contiguous; an ld* is the distance
  *     of two rows in elements (0: rows are dense), at most 2^20.  Nothing needs more alignment than its elements have;
  *     arrays whose rows start on 16 bytes and are whole multiples of 16 bytes long are read fastest.
  *   - the sums of products, the norms' sums and everything between two stores are float32 or wider; a stored value is rounded
@@ -320,7 +320,8 @@ typedef struct rt_gated_ffn {
     const void *w_gate, *w_up;   /* d_in x d_ff, both with stride ld_in */
     const void *w_down;          /* d_ff x d_out */
     void *out;                   /* T x d_out */
-    void *pre_gate, *pre_up;     /* T x d_ff: x w_gate and x w_up, kept for the backward pass; both NULL if there is none */
+    float *pre_gate, *pre_up;    /* T x d_ff float32 in every dtype: x w_gate and x w_up, kept for the backward pass (rounded
+                                    to 16 bits they would double the error of every gradient); both NULL if there is none */
 } rt_gated_ffn;
 
 /* Gradients of sum(dout * out).  A NULL output is not computed. */

@@ -14,6 +14,7 @@
 namespace {
 
 #include "rt_gemm.hpp"
+#include "rt_skinny.hpp"
 #include "rt_norm.hpp"
 
 int failf(rt_ctx* ctx, int code, const char* fmt, ...) {
@@ -54,24 +55,26 @@ struct Mat {
     const char* name;
     const void* p;
     int64_t rows, width, ld;      // ld in elements
+    int es;                       // bytes of an element
 };
 
 // Whether two matrices share an element.  Columns of one buffer (equal strides, disjoint column ranges) do not.
-bool overlap(const Mat& a, const Mat& b, int es) {
+bool overlap(const Mat& a, const Mat& b) {
     if (!a.p || !b.p || a.rows == 0 || b.rows == 0) return false;
-    const uintptr_t a0 = (uintptr_t)a.p, a1 = a0 + ((a.rows - 1) * a.ld + a.width) * es;
-    const uintptr_t b0 = (uintptr_t)b.p, b1 = b0 + ((b.rows - 1) * b.ld + b.width) * es;
+    const uintptr_t a0 = (uintptr_t)a.p, a1 = a0 + ((a.rows - 1) * a.ld + a.width) * a.es;
+    const uintptr_t b0 = (uintptr_t)b.p, b1 = b0 + ((b.rows - 1) * b.ld + b.width) * b.es;
     if (a1 <= b0 || b1 <= a0) return false;
-    if (a.ld != b.ld) return true;
-    const int64_t pitch = a.ld * es, d = (int64_t)(b0 - a0) % pitch, off = d < 0 ? d + pitch : d;
-    return !(off >= a.width * es && off + b.width * es <= pitch);
+    const int64_t pitch = a.ld * a.es;
+    if (pitch != b.ld * b.es) return true;
+    const int64_t d = (int64_t)(b0 - a0) % pitch, off = d < 0 ? d + pitch : d;
+    return !(off >= a.width * a.es && off + b.width * b.es <= pitch);
 }
 
 bool same_place(const Mat& a, const Mat& b) { return a.p == b.p && (a.ld == b.ld || a.rows <= 1); }
 
-int check_mat(rt_ctx* ctx, const char* fn, const Mat& m, int es, bool required) {
+int check_mat(rt_ctx* ctx, const char* fn, const Mat& m, bool required) {
     if (!m.p) return required && m.rows > 0 ? failf(ctx, RT_EINVAL, "%s: %s is NULL", fn, m.name) : RT_OK;
-    if ((uintptr_t)m.p % es) return failf(ctx, RT_EINVAL, "%s: %s is not aligned to its %d-byte elements", fn, m.name, es);
+    if ((uintptr_t)m.p % m.es) return failf(ctx, RT_EINVAL, "%s: %s is not aligned to its %d-byte elements", fn, m.name, m.es);
     if (m.ld < m.width)
         return failf(ctx, RT_EINVAL, "%s: the row stride of %s (%lld) is less than its width (%lld)", fn, m.name, (long long)m.ld,
                      (long long)m.width);
@@ -82,12 +85,12 @@ int check_mat(rt_ctx* ctx, const char* fn, const Mat& m, int es, bool required) 
 }
 
 // No output may share memory with an input or another output.
-int check_disjoint(rt_ctx* ctx, const char* fn, const Mat* in, int nin, const Mat* out, int nout, int es) {
+int check_disjoint(rt_ctx* ctx, const char* fn, const Mat* in, int nin, const Mat* out, int nout) {
     for (int i = 0; i < nout; ++i) {
         for (int j = 0; j < nin; ++j)
-            if (overlap(out[i], in[j], es)) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, in[j].name);
+            if (overlap(out[i], in[j])) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, in[j].name);
         for (int j = 0; j < i; ++j)
-            if (overlap(out[i], out[j], es)) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, out[j].name);
+            if (overlap(out[i], out[j])) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, out[j].name);
     }
     return RT_OK;
 }
@@ -108,11 +111,32 @@ struct Product {                // C [M x N] = X W over K, nseg segments, nbatch
 };
 
 struct Plan {
+    bool skinny;                // rt_skinny.hpp
     int bm, bn, splits, per_split, nk, tiles_m, tiles_n, nslot, Np;
     size_t part_bytes;
 };
 
+// Few rows against weights as they lie in memory: the weights' bytes are all the time there is.  Whether the kernel for
+// them can run depends on alignment too, so the workspace covers both.
+constexpr int SKINNY_ROWS = 32;
+bool skinny_sizes(const Product& p) { return p.M <= SKINNY_ROWS && p.lx == LK && p.lw == LI && p.N % 4 == 0; }
+
+void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
+    pl.skinny = true;
+    pl.nslot = p.epi == EPI_GATED ? 2 : 1;
+    pl.Np = p.N;
+    pl.tiles_n = (p.N + SK_COLS - 1) / SK_COLS;
+    // a second launch to join costs about as much as one CU takes to read 256 KB: workgroups that read less are not split
+    const int64_t steps = (p.K + 31) / 32, bytes = p.K * SK_COLS * elem_size(dtype) * pl.nslot;
+    int64_t s = 2 * cus / pl.tiles_n;
+    if (s > bytes >> 17) s = bytes >> 17;
+    if (s > steps / SK_WAVES) s = steps / SK_WAVES;
+    pl.splits = s < 1 ? 1 : (int)s;
+    pl.part_bytes = pl.splits > 1 ? (size_t)pl.splits * pl.nslot * p.M * pl.Np * sizeof(float) : 0;
+}
+
 int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, Plan& pl) {
+    pl.skinny = false;
     const int ke = 128 / elem_size(dtype);
     pl.bm = pl.bn = 128;
     const int cn = p.epi == EPI_GATED ? pl.bn / 2 : pl.bn;
@@ -142,6 +166,13 @@ GemmFn gemm_fn(bool al) {
     return al ? gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, true> : gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, false>;
 }
 
+int launch_join(rt_ctx* ctx, hipStream_t st, GemmFn join, int64_t M, int Np, int nbatch, const GemmArgs& a) {
+    const int64_t n = (M * (Np / 4) + 255) / 256;
+    hipLaunchKernelGGL(join, dim3((unsigned)(n < 8192 ? n : 8192), 1, nbatch), dim3(256), 0, st, a);
+    HIPCHK(ctx, hipGetLastError());
+    return RT_OK;
+}
+
 template <int DT>
 int launch_product(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a, bool al) {
     a.M = p.M; a.N = p.N; a.K = p.K; a.nseg = p.nseg; a.nk = pl.nk;
@@ -161,12 +192,25 @@ int launch_product(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl
     }
     hipLaunchKernelGGL(fn, dim3(pl.tiles_m * pl.tiles_n, pl.splits, p.nbatch), dim3(256), 0, st, a);
     HIPCHK(ctx, hipGetLastError());
-    if (pl.splits > 1) {
-        const int64_t n = (p.M * (pl.Np / 4) + 255) / 256;
-        hipLaunchKernelGGL(join, dim3((unsigned)(n < 8192 ? n : 8192), 1, p.nbatch), dim3(256), 0, st, a);
-        HIPCHK(ctx, hipGetLastError());
+    return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, p.nbatch, a) : RT_OK;
+}
+
+template <int DT>
+int launch_skinny(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a) {
+    a.M = p.M; a.N = p.N; a.K = p.K;
+    a.splits = pl.splits; a.Np = pl.Np; a.nslot = pl.nslot;
+    const bool two = p.M > 16;
+    GemmFn fn, join;
+    if (p.epi == EPI_GATED) {
+        fn = two ? skinny_kernel<DT, EPI_GATED, 2> : skinny_kernel<DT, EPI_GATED, 1>;
+        join = gemm_join_kernel<DT, EPI_GATED>;
+    } else {
+        fn = two ? skinny_kernel<DT, EPI_STORE, 2> : skinny_kernel<DT, EPI_STORE, 1>;
+        join = gemm_join_kernel<DT, EPI_STORE>;
     }
-    return RT_OK;
+    hipLaunchKernelGGL(fn, dim3(pl.tiles_n, pl.splits), dim3(64 * SK_WAVES), 0, st, a);
+    HIPCHK(ctx, hipGetLastError());
+    return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, 1, a) : RT_OK;
 }
 
 int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, GemmArgs& a) {
@@ -174,6 +218,12 @@ int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, Ge
     const int rc = plan_product(ctx, v.cu_count, dtype, p, pl);
     if (rc) return rc;
     const int es = elem_size(dtype), epc = 16 / es;
+    if (skinny_sizes(p) && a.ldw[0] % (4 * es) == 0 && (uintptr_t)a.w[0] % (4 * es) == 0 && (uintptr_t)a.w[1] % (4 * es) == 0) {
+        plan_skinny(v.cu_count, dtype, p, pl);
+        if (dtype == RT_F32) return launch_skinny<RT_F32>(ctx, v.stream, p, pl, a);
+        if (dtype == RT_BF16) return launch_skinny<RT_BF16>(ctx, v.stream, p, pl, a);
+        return launch_skinny<RT_F16>(ctx, v.stream, p, pl, a);
+    }
     bool al = (p.lx == LK ? p.K : p.M) % epc == 0 && (p.lw == LK ? p.K : p.N) % epc == 0 && a.ldx[0] % 16 == 0 && a.ldw[0] % 16 == 0;
     for (int i = 0; i < 2; ++i) al = al && (uintptr_t)a.x[i] % 16 == 0 && (uintptr_t)a.w[i] % 16 == 0;
     if (dtype == RT_F32) return launch_product<RT_F32>(ctx, v.stream, p, pl, a, al);
@@ -240,6 +290,12 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
         (rc = plan_product(ctx, cus, a.dtype, f.dw_in, f.pl_dw_in)) || (rc = plan_product(ctx, cus, a.dtype, f.dw_down, f.pl_dw_down)))
         return rc;
     f.ws_fwd = f.h_bytes + most(f.pl_gated.part_bytes, f.pl_down.part_bytes);
+    for (const Product* p : {&f.gated, &f.down})
+        if (skinny_sizes(*p)) {
+            Plan pl;
+            plan_skinny(cus, a.dtype, *p, pl);
+            f.ws_fwd = most(f.ws_fwd, f.h_bytes + pl.part_bytes);
+        }
     f.ws_bwd = 3 * f.h_bytes + most(most(f.pl_dh.part_bytes, f.pl_dx.part_bytes), most(f.pl_dw_in.part_bytes, f.pl_dw_down.part_bytes));
     return RT_OK;
 }
@@ -271,8 +327,8 @@ int ffn_forward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, char* ws) {
     set_x(g, a.x, a.x, a.ldx * es);
     set_w(g, a.w_gate, a.w_up, a.ld_in * es);
     set_o(g, 0, h, f.ldh * es);
-    set_o(g, 1, a.pre_gate, a.ld_pre * es);
-    set_o(g, 2, a.pre_up, a.ld_pre * es);
+    set_o(g, 1, a.pre_gate, a.ld_pre * 4);
+    set_o(g, 2, a.pre_up, a.ld_pre * 4);
     int rc = run_product(ctx, v, a.dtype, f.gated, g);
     if (rc) return rc;
     set_x(g, h, h, f.ldh * es);
@@ -299,7 +355,7 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
     set_o(g, 2, h, ldh);
     g.e[0] = (const char*)a.pre_gate;
     g.e[1] = (const char*)a.pre_up;
-    g.lde = a.ld_pre * es;
+    g.lde = a.ld_pre * 4;
     if ((rc = run_product(ctx, v, a.dtype, f.dh, g))) return rc;
     if (r.dx) {                      // dx = dgate Wg^T + dup Wu^T: one sum over both
         set_x(g, dg, du, ldh);
@@ -458,17 +514,17 @@ int rt_gated_ffn_dev(rt_ctx* ctx, const rt_gated_ffn* args, void* ws, size_t ws_
     int rc = ffn_make(ctx, fn, args, v.cu_count, f);
     if (rc) return rc;
     const rt_gated_ffn& a = f.a;
-    const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in},
-                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down}};
-    const Mat out[] = {{"out", a.out, a.T, a.d_out, a.ld_out}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre},
-                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre}, {"the workspace", ws, 1, (int64_t)(f.ws_fwd / f.es), (int64_t)(f.ws_fwd / f.es)}};
+    const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx, f.es}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in, f.es}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in, f.es},
+                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}};
+    const Mat out[] = {{"out", a.out, a.T, a.d_out, a.ld_out, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, 4},
+                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, 4}, {"the workspace", ws, 1, (int64_t)f.ws_fwd, (int64_t)f.ws_fwd, 1}};
     for (const Mat& m : in)
-        if ((rc = check_mat(ctx, fn, m, f.es, true))) return rc;
+        if ((rc = check_mat(ctx, fn, m, true))) return rc;
     for (int i = 0; i < 3; ++i)
-        if ((rc = check_mat(ctx, fn, out[i], f.es, i == 0))) return rc;
+        if ((rc = check_mat(ctx, fn, out[i], i == 0))) return rc;
     if (!a.pre_gate != !a.pre_up) return failf(ctx, RT_EINVAL, "%s: give both of pre_gate and pre_up, or neither", fn);
     if (a.T == 0) return RT_OK;
-    if ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_fwd)) || (rc = check_disjoint(ctx, fn, in, 4, out, 4, f.es))) return rc;
+    if ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_fwd)) || (rc = check_disjoint(ctx, fn, in, 4, out, 4))) return rc;
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);
     return ffn_forward(ctx, v, f, (char*)ws);
@@ -489,18 +545,18 @@ int rt_gated_ffn_backward_dev(rt_ctx* ctx, const rt_gated_ffn* args, const rt_ga
     if (!r.ld_dx) r.ld_dx = a.d_in;
     if (!r.ld_dw_in) r.ld_dw_in = a.d_ff;
     if (!r.ld_dw_down) r.ld_dw_down = a.d_out;
-    const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in},
-                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre},
-                      {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre}, {"dout", r.dout, a.T, a.d_out, r.ld_dout}};
-    const Mat out[] = {{"dx", r.dx, a.T, a.d_in, r.ld_dx}, {"dw_gate", r.dw_gate, a.d_in, a.d_ff, r.ld_dw_in},
-                       {"dw_up", r.dw_up, a.d_in, a.d_ff, r.ld_dw_in}, {"dw_down", r.dw_down, a.d_ff, a.d_out, r.ld_dw_down},
-                       {"the workspace", ws, 1, (int64_t)(f.ws_bwd / f.es), (int64_t)(f.ws_bwd / f.es)}};
+    const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx, f.es}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in, f.es}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in, f.es},
+                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, 4},
+                      {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, 4}, {"dout", r.dout, a.T, a.d_out, r.ld_dout, f.es}};
+    const Mat out[] = {{"dx", r.dx, a.T, a.d_in, r.ld_dx, f.es}, {"dw_gate", r.dw_gate, a.d_in, a.d_ff, r.ld_dw_in, f.es},
+                       {"dw_up", r.dw_up, a.d_in, a.d_ff, r.ld_dw_in, f.es}, {"dw_down", r.dw_down, a.d_ff, a.d_out, r.ld_dw_down, f.es},
+                       {"the workspace", ws, 1, (int64_t)f.ws_bwd, (int64_t)f.ws_bwd, 1}};
     for (const Mat& m : in)
-        if ((rc = check_mat(ctx, fn, m, f.es, true))) return rc;
+        if ((rc = check_mat(ctx, fn, m, true))) return rc;
     for (int i = 0; i < 4; ++i)
-        if ((rc = check_mat(ctx, fn, out[i], f.es, false))) return rc;
+        if ((rc = check_mat(ctx, fn, out[i], false))) return rc;
     if (a.T > 0 && ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_bwd)))) return rc;
-    if ((rc = check_disjoint(ctx, fn, in, 7, out, a.T > 0 ? 5 : 4, f.es))) return rc;
+    if ((rc = check_disjoint(ctx, fn, in, 7, out, a.T > 0 ? 5 : 4))) return rc;
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);
     if (a.T == 0) {
@@ -534,22 +590,22 @@ int rt_block_norm_dev(rt_ctx* ctx, const rt_block_norm* args) {
     if (rc) return rc;
     const rt_block_norm& a = m.a;
     const int64_t gates = (a.T + a.rows_per_gate - 1) / a.rows_per_gate;
-    const Mat in[] = {{"x", a.x, a.T, a.d, a.ldx}, {"branch", a.branch, a.T, a.d, a.ld_branch}, {"gate", a.gate, gates, a.d, a.ld_gate},
-                      {"w_post", a.w_post, 1, a.d, a.d}, {"w_pre", a.w_pre, 1, a.d, a.d}};
-    const Mat out[] = {{"y", a.y, a.T, a.d, a.ldy}, {"n", a.n, a.T, a.d, a.ldn}};
+    const Mat in[] = {{"x", a.x, a.T, a.d, a.ldx, m.es}, {"branch", a.branch, a.T, a.d, a.ld_branch, m.es}, {"gate", a.gate, gates, a.d, a.ld_gate, m.es},
+                      {"w_post", a.w_post, 1, a.d, a.d, m.es}, {"w_pre", a.w_pre, 1, a.d, a.d, m.es}};
+    const Mat out[] = {{"y", a.y, a.T, a.d, a.ldy, m.es}, {"n", a.n, a.T, a.d, a.ldn, m.es}};
     for (int i = 0; i < 5; ++i)
-        if ((rc = check_mat(ctx, fn, in[i], m.es, i == 0))) return rc;
+        if ((rc = check_mat(ctx, fn, in[i], i == 0))) return rc;
     for (const Mat& o : out)
-        if ((rc = check_mat(ctx, fn, o, m.es, false))) return rc;
+        if ((rc = check_mat(ctx, fn, o, false))) return rc;
     if (a.gate && !a.branch) return failf(ctx, RT_EINVAL, "%s: a gate without a branch", fn);
     if (a.T == 0) return RT_OK;
     if (!a.y && !a.n) return failf(ctx, RT_EINVAL, "%s: y and n are both NULL", fn);
     // rows are read before they are written: an output may take the place of x or of branch, whole
     for (const Mat& o : out)
         for (int i = 0; i < 5; ++i)
-            if (overlap(o, in[i], m.es) && !(i < 2 && same_place(o, in[i])))
+            if (overlap(o, in[i]) && !(i < 2 && same_place(o, in[i])))
                 return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, o.name, in[i].name);
-    if (overlap(out[0], out[1], m.es)) return failf(ctx, RT_EINVAL, "%s: y and n overlap", fn);
+    if (overlap(out[0], out[1])) return failf(ctx, RT_EINVAL, "%s: y and n overlap", fn);
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);
     NormArgs k;
@@ -580,16 +636,16 @@ int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_
     const int64_t gates = (a.T + a.rows_per_gate - 1) / a.rows_per_gate;
     // without a branch y is res_scale * x, and x stands in for a y that was not written
     const bool from_x = !a.y && !a.branch;
-    const Mat yin = from_x ? Mat{"x", a.x, a.T, a.d, a.ldx} : Mat{"y", a.y, a.T, a.d, a.ldy};
-    const Mat in[] = {yin, {"branch", a.branch, a.T, a.d, a.ld_branch}, {"dy", r.dy, a.T, a.d, r.ld_dy}, {"dn", r.dn, a.T, a.d, r.ld_dn},
-                      {"gate", a.gate, gates, a.d, a.ld_gate}, {"w_post", a.w_post, 1, a.d, a.d}, {"w_pre", a.w_pre, 1, a.d, a.d}};
-    const Mat out[] = {{"dx", r.dx, a.T, a.d, r.ld_dx}, {"dbranch", r.dbranch, a.T, a.d, r.ld_dbranch}, {"dgate", r.dgate, gates, a.d, r.ld_dgate},
-                       {"dw_post", r.dw_post, 1, a.d, a.d}, {"dw_pre", r.dw_pre, 1, a.d, a.d},
-                       {"the workspace", ws, 1, (int64_t)(m.ws / m.es), (int64_t)(m.ws / m.es)}};
+    const Mat yin = from_x ? Mat{"x", a.x, a.T, a.d, a.ldx, m.es} : Mat{"y", a.y, a.T, a.d, a.ldy, m.es};
+    const Mat in[] = {yin, {"branch", a.branch, a.T, a.d, a.ld_branch, m.es}, {"dy", r.dy, a.T, a.d, r.ld_dy, m.es}, {"dn", r.dn, a.T, a.d, r.ld_dn, m.es},
+                      {"gate", a.gate, gates, a.d, a.ld_gate, m.es}, {"w_post", a.w_post, 1, a.d, a.d, m.es}, {"w_pre", a.w_pre, 1, a.d, a.d, m.es}};
+    const Mat out[] = {{"dx", r.dx, a.T, a.d, r.ld_dx, m.es}, {"dbranch", r.dbranch, a.T, a.d, r.ld_dbranch, m.es}, {"dgate", r.dgate, gates, a.d, r.ld_dgate, m.es},
+                       {"dw_post", r.dw_post, 1, a.d, a.d, m.es}, {"dw_pre", r.dw_pre, 1, a.d, a.d, m.es},
+                       {"the workspace", ws, 1, (int64_t)m.ws, (int64_t)m.ws, 1}};
     for (int i = 0; i < 7; ++i)
-        if ((rc = check_mat(ctx, fn, in[i], m.es, i == 0 && r.dn))) return rc;
+        if ((rc = check_mat(ctx, fn, in[i], i == 0 && r.dn))) return rc;
     for (int i = 0; i < 5; ++i)
-        if ((rc = check_mat(ctx, fn, out[i], m.es, false))) return rc;
+        if ((rc = check_mat(ctx, fn, out[i], false))) return rc;
     if (a.T > 0 && !r.dy && !r.dn) return failf(ctx, RT_EINVAL, "%s: dy and dn are both NULL", fn);
     if (a.gate && !a.branch) return failf(ctx, RT_EINVAL, "%s: a gate without a branch", fn);
     if (!a.branch && (r.dbranch || r.dgate || r.dw_post)) return failf(ctx, RT_EINVAL, "%s: dbranch, dgate or dw_post without a branch", fn);
@@ -599,10 +655,10 @@ int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_
     for (int i = 0; i < (a.T > 0 ? 6 : 5); ++i) {
         for (int j = 0; j < 7; ++j) {
             const bool fine = same_place(out[i], in[j]) && ((i == 0 && (j == 0 || j == 2 || j == 3)) || (i == 1 && j < 4));
-            if (overlap(out[i], in[j], m.es) && !fine) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, in[j].name);
+            if (overlap(out[i], in[j]) && !fine) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, in[j].name);
         }
         for (int j = 0; j < i; ++j)
-            if (overlap(out[i], out[j], m.es)) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, out[j].name);
+            if (overlap(out[i], out[j])) return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, out[i].name, out[j].name);
     }
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);

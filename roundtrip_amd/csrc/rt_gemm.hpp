@@ -24,9 +24,9 @@ struct GemmArgs {
     int splits, per_split;         // K tiles are dealt to blockIdx.y, per_split each
     float* part;                   // splits > 1: [split][slot][M][Np] partial sums, joined by gemm_join_kernel
     int Np, nslot;
-    char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two may be NULL).
+    char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two float32 or NULL).
     long long ldo[3];              // EPI_GATED_BWD: dgate, dup, h
-    const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept
+    const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept, float32
     long long lde;
     int act;
     float alpha;
@@ -79,11 +79,11 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, 
         }
         store4<DT>(a.o[0] + m * a.ldo[0] + c, h, valid);
         if (a.o[1]) {
-            store4<DT>(a.o[1] + m * a.ldo[1] + c, v0, valid);
-            store4<DT>(a.o[2] + m * a.ldo[2] + c, v1, valid);
+            store4<RT_F32>(a.o[1] + m * a.ldo[1] + n * 4ll, v0, valid);
+            store4<RT_F32>(a.o[2] + m * a.ldo[2] + n * 4ll, v1, valid);
         }
     } else {
-        const f32x4 g = load4<DT>(a.e[0] + m * a.lde + c, valid), u = load4<DT>(a.e[1] + m * a.lde + c, valid);
+        const f32x4 g = load4<RT_F32>(a.e[0] + m * a.lde + n * 4ll, valid), u = load4<RT_F32>(a.e[1] + m * a.lde + n * 4ll, valid);
         f32x4 dg, du, h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

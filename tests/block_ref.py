@@ -57,7 +57,7 @@ def gated(x, wg, wu, kind, alpha, dtype):
 def ffn(x, wg, wu, wd, kind, alpha, dtype):
     (g, eg), (u, eu), (h, eh) = gated(x, wg, wu, kind, alpha, dtype)
     out = rounded(*mm(*rounded(h, eh, dtype), wd), dtype)
-    return {"out": out, "pre_gate": rounded(g, eg, dtype), "pre_up": rounded(u, eu, dtype)}
+    return {"out": out, "pre_gate": (g, eg), "pre_up": (u, eu)}
 
 
 def ffn_back(x, wg, wu, wd, g, u, dout, kind, alpha, dtype):

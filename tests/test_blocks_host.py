@@ -64,7 +64,7 @@ WS = C.c_void_p(BASE + (1 << 30))
     (dict(ld_down=(1 << 20) + 8), EUNSUPPORTED, "row stride of w_down"), (dict(pre_gate=BASE + (1 << 28)), EINVAL, "both of pre_gate"),
     (dict(pre_up=BASE + (1 << 28)), EINVAL, "both of pre_gate"), (dict(out=BASE), EINVAL, "out and x overlap"),
     (dict(out=BASE + 318), EINVAL, "out and x overlap"), (dict(out=BASE + (1 << 24) + 64), EINVAL, "out and w_gate overlap"),
-    (dict(pre_gate=BASE + (1 << 28), pre_up=BASE + (1 << 28) + 2), EINVAL, "overlap"), (dict(out=WS.value), EINVAL, "workspace and out overlap"),
+    (dict(pre_gate=BASE + (1 << 28), pre_up=BASE + (1 << 28) + 4), EINVAL, "overlap"), (dict(pre_gate=BASE + (1 << 28) + 2, pre_up=BASE + (1 << 27)), EINVAL, "pre_gate is not aligned"), (dict(out=WS.value), EINVAL, "workspace and out overlap"),
     (dict(T=1 << 38, d_ff=1 << 20, d_in=1 << 20), EUNSUPPORTED, "one launch")])
 def test_gated_ffn_refusals(lib, kw, code, words):
     a = ffn(**kw)
@@ -157,9 +157,9 @@ def test_block_norm_workspace_is_asked_for(lib):
 def test_columns_of_one_buffer_do_not_overlap(lib):
     """Gate and up, and what is kept of them, as the halves of one array: past every check (the call then needs a GPU, or the
     workspace that is refused here)."""
-    a = ffn(w_up=BASE + (1 << 24) + 64, ld_in=64, pre_gate=BASE + (1 << 28), pre_up=BASE + (1 << 28) + 64, ld_pre=64)
+    a = ffn(w_up=BASE + (1 << 24) + 64, ld_in=64, pre_gate=BASE + (1 << 28), pre_up=BASE + (1 << 28) + 128, ld_pre=64)
     refused(lib, lib.rt_gated_ffn_dev(lib.ctx, C.byref(a), None, 0), EINVAL, "workspace is NULL")
-    shifted = ffn(pre_gate=BASE + (1 << 28), pre_up=BASE + (1 << 28) + 62, ld_pre=64)
+    shifted = ffn(pre_gate=BASE + (1 << 28), pre_up=BASE + (1 << 28) + 124, ld_pre=64)
     refused(lib, lib.rt_gated_ffn_dev(lib.ctx, C.byref(shifted), WS, 1 << 62), EINVAL, "pre_up and pre_gate overlap")
 
 

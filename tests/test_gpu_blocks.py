@@ -58,7 +58,8 @@ def ffn_case(engine, T, di, f, do, dt, act, lds=(0, 0, 0, 0, 0), shift=0, alpha=
     ld = [w + l for w, l in zip((di, f, do, do, f), lds)]
     A = lambda r, w, l=None, v=None: Array(r, w, dtype, l, shift, v)  # noqa: E731
     ax, ag, au, ad = A(T, di, ld[0], x), A(di, f, ld[1], wg), A(di, f, ld[1], wu), A(f, do, ld[2], wd)
-    ao, pg, pu, ado = A(T, do, ld[3]), A(T, f, ld[4]), A(T, f, ld[4]), A(T, do, ld[3], dout)
+    ao, ado = A(T, do, ld[3]), A(T, do, ld[3], dout)
+    pg, pu = Array(T, f, torch.float32, ld[4], shift), Array(T, f, torch.float32, ld[4], shift)
     for keep in (False, True):
         a = engine.gated_ffn_args(T, di, f, do, CODE[dt], ACT[act], x=ax.ptr, w_gate=ag.ptr, w_up=au.ptr, w_down=ad.ptr,
                                   out=ao.ptr, pre_gate=pg.ptr if keep else None, pre_up=pu.ptr if keep else None, alpha=alpha,
@@ -80,8 +81,8 @@ def ffn_case(engine, T, di, f, do, dt, act, lds=(0, 0, 0, 0, 0), shift=0, alpha=
             assert arr.untouched_outside()
     assert torch.equal(first, ao.view)                   # keeping the gate and up changes nothing
     # backward, at values of pre_gate and pre_up of its own
-    g, g64 = normal(gen, (T, f), dtype, 1.5)
-    u, u64 = normal(gen, (T, f), dtype)
+    g, g64 = normal(gen, (T, f), torch.float32, 1.5)
+    u, u64 = normal(gen, (T, f), torch.float32)
     pg.view.copy_(g)
     pu.view.copy_(u)
     dx, dg, du, dd = A(T, di, ld[0]), A(di, f, ld[1]), A(di, f, ld[1]), A(f, do, ld[2])
@@ -163,9 +164,9 @@ def test_gated_ffn_weights_side_by_side(engine):
     wd, wd64 = normal(gen, (f, di), dtype, 0.1)
     xd, wc, wdd = x.cuda(), w.cuda(), wd.cuda()
     out = torch.empty(T, di, dtype=dtype, device="cuda")
-    pre = torch.empty(T, 2 * f, dtype=dtype, device="cuda")
+    pre = torch.empty(T, 2 * f, device="cuda")
     a = engine.gated_ffn_args(T, di, f, di, CODE["bf16"], ACT["silu"], x=xd.data_ptr(), w_gate=wc.data_ptr(), w_up=wc.data_ptr() + 2 * f,
-                              w_down=wdd.data_ptr(), out=out.data_ptr(), pre_gate=pre.data_ptr(), pre_up=pre.data_ptr() + 2 * f,
+                              w_down=wdd.data_ptr(), out=out.data_ptr(), pre_gate=pre.data_ptr(), pre_up=pre.data_ptr() + 4 * f,
                               ld_in=2 * f, ld_pre=2 * f)
     n = max(engine.gated_ffn_workspace(a), engine.gated_ffn_workspace(a, True))
     ws = workspace(n)
@@ -411,7 +412,7 @@ class Block(object):
                      "w_pre": normal(gen, (d,), self.dtype, 0.1, 1.0), "gate": normal(gen, (-(-T // 3), d), self.dtype, 0.5),
                      "dy": normal(gen, (T, d), self.dtype), "dn": normal(gen, (T, d), self.dtype)}
         t = self.t = {k: v[0].cuda() for k, v in self.host.items()}
-        t.update(h=new(T, d), b=new(T, d), y=new(T, d), n=new(T, d), pg=new(T, f), pu=new(T, f), dx=new(T, d), db=new(T, d), dh=new(T, d))
+        t.update(h=new(T, d), b=new(T, d), y=new(T, d), n=new(T, d), pg=torch.empty(T, f, device="cuda"), pu=torch.empty(T, f, device="cuda"), dx=new(T, d), db=new(T, d), dh=new(T, d))
         for k in ("w_in", "w_gate", "w_up", "w_down", "w_post", "w_pre", "gate"):
             t["d" + k] = torch.empty_like(t[k])
         p = {k: v.data_ptr() for k, v in t.items()}
@@ -462,7 +463,7 @@ def exact_block(host):
 @pytest.mark.parametrize("T,d,f", [(1, 64, 128), (50, 128, 320), (200, 90, 170)])
 def test_block_together(engine, T, d, f, dt):
     """Forward and backward in a row against float64.  Between two operators a value is rounded once: nine roundings lie on
-    the longest way (h, gate and up, the product, b, y; then db, dg / du, dh, the result), each off by at most u of its size and
+    the longest way at most (the norm's h, the product's h, b, y; then db, dg, du, dh, the result), each off by at most u of its size and
     nearly independent from element to element, so each moves a result by at most about u of its root mean square; norms and
     activations stretch a relative error by less than 2 here, hence 2 * 9 u in that measure."""
     blk = Block(engine, T, d, f, dt)
