@@ -112,24 +112,33 @@ struct Product {                // C [M x N] = X W over K, nseg segments, nbatch
 
 struct Plan {
     bool skinny;                // rt_skinny.hpp
+    int li;
     int bm, bn, splits, per_split, nk, tiles_m, tiles_n, nslot, Np;
     size_t part_bytes;
 };
 
 // Few rows against weights as they lie in memory: the weights' bytes are all the time there is.  Whether the kernel for
 // them can run depends on alignment too, so the workspace covers both.
-constexpr int SKINNY_ROWS = 32;
+constexpr int SKINNY_ROWS = 32, GEMV_ROWS = 4;
 bool skinny_sizes(const Product& p) { return p.M <= SKINNY_ROWS && p.lx == LK && p.lw == LI && p.N % 4 == 0; }
 
 void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
+    const int es = elem_size(dtype);
     pl.skinny = true;
     pl.nslot = p.epi == EPI_GATED ? 2 : 1;
     pl.Np = p.N;
-    pl.tiles_n = (p.N + SK_COLS - 1) / SK_COLS;
-    // a second launch to join costs about as much as one CU takes to read 256 KB: workgroups that read less are not split
-    const int64_t steps = (p.K + 31) / 32, bytes = p.K * SK_COLS * elem_size(dtype) * pl.nslot;
-    int64_t s = 2 * cus / pl.tiles_n;
-    if (s > bytes >> 17) s = bytes >> 17;
+    // Lanes of a row (gemv_kernel): 16 where that gives every CU a slab, or where there is so much to read that lines should
+    // be read whole by one workgroup (32 MB: 6 us of the chip); else as few as give more workgroups.
+    const int64_t all = p.K * p.N * es * pl.nslot;
+    pl.li = 16;
+    if (p.M <= GEMV_ROWS && all < (32 << 20))
+        while (pl.li > 4 && p.N / (4 * pl.li) < cus) pl.li /= 2;
+    const int cols = 4 * pl.li;
+    pl.tiles_n = (p.N + cols - 1) / cols;
+    // K is split where columns alone leave CUs idle.  A second launch to join the splits costs about 4 us, in which one CU reads
+    // some 256 KB: workgroups that read less than twice that are not split.
+    const int64_t steps = (p.K + 31) / 32, bytes = p.K * cols * es * pl.nslot;
+    int64_t s = bytes >= (512 << 10) ? cus / pl.tiles_n : 1;
     if (s > steps / SK_WAVES) s = steps / SK_WAVES;
     pl.splits = s < 1 ? 1 : (int)s;
     pl.part_bytes = pl.splits > 1 ? (size_t)pl.splits * pl.nslot * p.M * pl.Np * sizeof(float) : 0;
@@ -167,8 +176,11 @@ GemmFn gemm_fn(bool al) {
 }
 
 int launch_join(rt_ctx* ctx, hipStream_t st, GemmFn join, int64_t M, int Np, int nbatch, const GemmArgs& a) {
-    const int64_t n = (M * (Np / 4) + 255) / 256;
-    hipLaunchKernelGGL(join, dim3((unsigned)(n < 8192 ? n : 8192), 1, nbatch), dim3(256), 0, st, a);
+    // small joins: one wave a workgroup, so that they spread over the CUs
+    const int64_t quads = M * (Np / 4);
+    const int threads = quads < 65536 ? 64 : 256;
+    const int64_t n = (quads + threads - 1) / threads;
+    hipLaunchKernelGGL(join, dim3((unsigned)(n < 8192 ? n : 8192), 1, nbatch), dim3(threads), 0, st, a);
     HIPCHK(ctx, hipGetLastError());
     return RT_OK;
 }
@@ -195,19 +207,26 @@ int launch_product(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl
     return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, p.nbatch, a) : RT_OK;
 }
 
+template <int DT, int EPI, int MR>
+GemmFn gemv_fn(int li) {
+    return li == 16 ? gemv_kernel<DT, EPI, MR, 16> : li == 8 ? gemv_kernel<DT, EPI, MR, 8> : gemv_kernel<DT, EPI, MR, 4>;
+}
+
+template <int DT, int EPI>
+GemmFn skinny_fn(int64_t M, int li) {
+    if (M == 1) return gemv_fn<DT, EPI, 1>(li);
+    if (M == 2) return gemv_fn<DT, EPI, 2>(li);
+    if (M <= GEMV_ROWS) return gemv_fn<DT, EPI, GEMV_ROWS>(li);
+    return M <= 16 ? skinny_kernel<DT, EPI, 1> : skinny_kernel<DT, EPI, 2>;
+}
+
 template <int DT>
 int launch_skinny(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a) {
     a.M = p.M; a.N = p.N; a.K = p.K;
     a.splits = pl.splits; a.Np = pl.Np; a.nslot = pl.nslot;
-    const bool two = p.M > 16;
-    GemmFn fn, join;
-    if (p.epi == EPI_GATED) {
-        fn = two ? skinny_kernel<DT, EPI_GATED, 2> : skinny_kernel<DT, EPI_GATED, 1>;
-        join = gemm_join_kernel<DT, EPI_GATED>;
-    } else {
-        fn = two ? skinny_kernel<DT, EPI_STORE, 2> : skinny_kernel<DT, EPI_STORE, 1>;
-        join = gemm_join_kernel<DT, EPI_STORE>;
-    }
+    const bool gated = p.epi == EPI_GATED;
+    const GemmFn fn = gated ? skinny_fn<DT, EPI_GATED>(p.M, pl.li) : skinny_fn<DT, EPI_STORE>(p.M, pl.li);
+    const GemmFn join = gated ? gemm_join_kernel<DT, EPI_GATED> : gemm_join_kernel<DT, EPI_STORE>;
     hipLaunchKernelGGL(fn, dim3(pl.tiles_n, pl.splits), dim3(64 * SK_WAVES), 0, st, a);
     HIPCHK(ctx, hipGetLastError());
     return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, 1, a) : RT_OK;
@@ -385,7 +404,8 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
 struct Norm {
     rt_block_norm a;
     int es;
-    int tpr;                         // threads of a row
+    int tpr, tpr_back;               // threads of a row
+    int together;
     int units;
     int64_t rows_per_unit;
     size_t part, ws;                 // bytes of one [units][d] array; of the workspace
@@ -414,12 +434,24 @@ int norm_make(rt_ctx* ctx, const char* fn, const rt_block_norm* in, int cus, Nor
     if (a.T > 0x7fffffffll)
         return failf(ctx, RT_EUNSUPPORTED, "%s: T = %lld rows are more than one launch covers", fn, (long long)a.T);
     const int chunks = (a.d + 16 / m.es - 1) / (16 / m.es);
-    m.tpr = chunks <= 256 ? 64 : chunks <= 1024 ? 256 : 1024;
-    // units: enough to fill the chip, consecutive rows each; whole gate groups where a unit can hold some
-    const int64_t fill = (int64_t)cus * (m.tpr == 64 ? 16 : m.tpr == 256 ? 4 : 1);
+    // A row to a wave where it is short; with fewer rows than CUs, to a workgroup sooner (a chunk a thread: what counts is
+    // how long one row takes)
+    const bool few = a.T < cus;
+    m.tpr = chunks <= (few ? 64 : 256) ? 64 : chunks <= 1024 ? 256 : 1024;
+    // backward: five arrays and three sums of a chunk of eight values are about what a thread's registers hold; two chunks of
+    // four float32 values
+    const int per = a.dtype == RT_F32 ? 2 : 1;
+    m.tpr_back = chunks <= 64 * (few ? 1 : per) ? 64 : chunks <= 256 * per ? 256 : chunks <= 1024 ? 512 : 1024;
+    // units: as many workgroups a CU as their registers allow, consecutive rows each; whole gates where a unit can hold some
+    const int64_t fill = (int64_t)cus * (m.tpr_back >= 512 ? 1 : 2);
     int64_t r = (a.T + fill - 1) / fill;
+    const int waves = m.tpr_back == 64 ? 4 : 1;
+    if (m.tpr_back == 64 && r < waves) r = waves;
+    // a wave walks four gates at least before a segment's end is worth an exchange between waves
+    m.together = a.rows_per_gate >= 16;
+    if (a.gate && waves > 1 && !m.together) r = up(r, waves * a.rows_per_gate);
+    else if (a.gate && a.rows_per_gate <= r) r = r / a.rows_per_gate * a.rows_per_gate;
     if (r < 1) r = 1;
-    if (a.gate && a.rows_per_gate <= r) r = r / a.rows_per_gate * a.rows_per_gate;
     m.rows_per_unit = r;
     m.units = (int)((a.T + r - 1) / r);
     m.part = (size_t)m.units * a.d * sizeof(float);
@@ -428,34 +460,43 @@ int norm_make(rt_ctx* ctx, const char* fn, const rt_block_norm* in, int cus, Nor
 }
 
 template <int DT, bool AL, int TPR, int NV>
-void launch_norm(hipStream_t st, const NormArgs& a, int what) {
+void launch_norm(hipStream_t st, const NormArgs& a) {
     constexpr int B = norm_block(TPR), RPB = B / TPR;
-    if (what == 0)
-        hipLaunchKernelGGL((norm_kernel<DT, TPR, NV, AL>), dim3((unsigned)((a.T + RPB - 1) / RPB)), dim3(B), 0, st, a);
-    else
-        hipLaunchKernelGGL((norm_back_kernel<DT, TPR, NV, AL>), dim3((unsigned)((a.units + RPB - 1) / RPB)), dim3(B), 0, st, a);
+    hipLaunchKernelGGL((norm_kernel<DT, TPR, NV, AL>), dim3((unsigned)((a.T + RPB - 1) / RPB)), dim3(B), 0, st, a);
+}
+
+template <int DT, bool AL, int TPR, int NV>
+void launch_norm_back(hipStream_t st, const NormArgs& a) {
+    hipLaunchKernelGGL((norm_back_kernel<DT, TPR, NV, AL>), dim3((unsigned)a.units), dim3(norm_block(TPR)), 0, st, a);
 }
 
 template <int DT, bool AL>
-void pick_norm(hipStream_t st, const NormArgs& a, int tpr, int what) {
+void pick_norm(hipStream_t st, const NormArgs& a, int tpr, bool back) {
     const int nv = ((a.d + EPC<DT> - 1) / EPC<DT> + tpr - 1) / tpr;
-    if (tpr == 64) {
-        if (nv <= 1) launch_norm<DT, AL, 64, 1>(st, a, what);
-        else if (nv <= 2) launch_norm<DT, AL, 64, 2>(st, a, what);
-        else launch_norm<DT, AL, 64, 4>(st, a, what);
+    if (back) {
+        constexpr int PER = DT == RT_F32 ? 2 : 1;
+        if (tpr == 64) nv <= 1 ? launch_norm_back<DT, AL, 64, 1>(st, a) : launch_norm_back<DT, AL, 64, PER>(st, a);
+        else if (tpr == 256) nv <= 1 ? launch_norm_back<DT, AL, 256, 1>(st, a) : launch_norm_back<DT, AL, 256, PER>(st, a);
+        else if (tpr == 512) nv <= 1 ? launch_norm_back<DT, AL, 512, 1>(st, a) : launch_norm_back<DT, AL, 512, 2>(st, a);
+        else if (nv <= 2) launch_norm_back<DT, AL, 1024, 2>(st, a);
+        else launch_norm_back<DT, AL, 1024, 4>(st, a);
+    } else if (tpr == 64) {
+        if (nv <= 1) launch_norm<DT, AL, 64, 1>(st, a);
+        else if (nv <= 2) launch_norm<DT, AL, 64, 2>(st, a);
+        else launch_norm<DT, AL, 64, 4>(st, a);
     } else if (tpr == 256) {
-        if (nv <= 2) launch_norm<DT, AL, 256, 2>(st, a, what);
-        else launch_norm<DT, AL, 256, 4>(st, a, what);
+        if (nv <= 1) launch_norm<DT, AL, 256, 1>(st, a);
+        else if (nv <= 2) launch_norm<DT, AL, 256, 2>(st, a);
+        else launch_norm<DT, AL, 256, 4>(st, a);
     } else {
-        if (nv <= 2) launch_norm<DT, AL, 1024, 2>(st, a, what);
-        else launch_norm<DT, AL, 1024, 4>(st, a, what);
+        nv <= 2 ? launch_norm<DT, AL, 1024, 2>(st, a) : launch_norm<DT, AL, 1024, 4>(st, a);
     }
 }
 
-int run_norm(rt_ctx* ctx, hipStream_t st, int dtype, const NormArgs& a, int tpr, int what, bool al) {
-    if (dtype == RT_F32) al ? pick_norm<RT_F32, true>(st, a, tpr, what) : pick_norm<RT_F32, false>(st, a, tpr, what);
-    else if (dtype == RT_BF16) al ? pick_norm<RT_BF16, true>(st, a, tpr, what) : pick_norm<RT_BF16, false>(st, a, tpr, what);
-    else al ? pick_norm<RT_F16, true>(st, a, tpr, what) : pick_norm<RT_F16, false>(st, a, tpr, what);
+int run_norm(rt_ctx* ctx, hipStream_t st, int dtype, const NormArgs& a, int tpr, bool back, bool al) {
+    if (dtype == RT_F32) al ? pick_norm<RT_F32, true>(st, a, tpr, back) : pick_norm<RT_F32, false>(st, a, tpr, back);
+    else if (dtype == RT_BF16) al ? pick_norm<RT_BF16, true>(st, a, tpr, back) : pick_norm<RT_BF16, false>(st, a, tpr, back);
+    else al ? pick_norm<RT_F16, true>(st, a, tpr, back) : pick_norm<RT_F16, false>(st, a, tpr, back);
     HIPCHK(ctx, hipGetLastError());
     return RT_OK;
 }
@@ -614,7 +655,7 @@ int rt_block_norm_dev(rt_ctx* ctx, const rt_block_norm* args) {
     al.es = m.es;
     for (const Mat& x : in) al(x.p, x.ld, x.width);
     for (const Mat& x : out) al(x.p, x.ld, x.width);
-    return run_norm(ctx, v.stream, a.dtype, k, m.tpr, 0, al.ok);
+    return run_norm(ctx, v.stream, a.dtype, k, m.tpr, false, al.ok);
 }
 
 int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_block_norm_grads* grads, void* ws, size_t ws_bytes) {
@@ -674,23 +715,23 @@ int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_
     k.dx = (char*)r.dx; k.db = (char*)r.dbranch; k.dgate = (char*)r.dgate;
     k.lddy = r.ld_dy * es; k.lddn = r.ld_dn * es; k.lddx = r.ld_dx * es; k.lddb = r.ld_dbranch * es; k.lddg = r.ld_dgate * es;
     k.want_post = r.dw_post != nullptr; k.want_pre = r.dw_pre != nullptr && r.dn != nullptr;
-    k.rows_per_unit = m.rows_per_unit; k.units = m.units;
+    k.rows_per_unit = m.rows_per_unit; k.units = m.units; k.together = m.together;
     k.p_post = (float*)ws; k.p_pre = (float*)((char*)ws + m.part); k.p_gate = (float*)((char*)ws + 2 * m.part);
     k.dw_post = (char*)r.dw_post; k.dw_pre = k.want_pre ? (char*)r.dw_pre : nullptr;
     Aligned al;
     al.es = m.es;
     for (const Mat& x : in) al(x.p, x.ld, x.width);
     for (int i = 0; i < 5; ++i) al(out[i].p, out[i].ld, out[i].width);
-    if ((rc = run_norm(ctx, v.stream, a.dtype, k, m.tpr, 1, al.ok))) return rc;
+    if ((rc = run_norm(ctx, v.stream, a.dtype, k, m.tpr_back, true, al.ok))) return rc;
     if (r.dw_pre && !r.dn && (rc = zero_rows(ctx, v.stream, r.dw_pre, (int64_t)a.d * es, 1, (int64_t)a.d * es))) return rc;
     // what is left to join: the weights' sums, and the gates that more than one unit saw
     const bool gates_left = r.dgate && a.rows_per_gate > m.rows_per_unit;
     const int first = k.want_post || k.want_pre ? 0 : 2, last = gates_left ? 2 + (int)gates : 2;
     if (last > first) {
         const dim3 grid((a.d + 31) / 32, last - first);
-        if (a.dtype == RT_F32) hipLaunchKernelGGL(norm_join_kernel<RT_F32>, grid, dim3(256), 0, v.stream, k, first);
-        else if (a.dtype == RT_BF16) hipLaunchKernelGGL(norm_join_kernel<RT_BF16>, grid, dim3(256), 0, v.stream, k, first);
-        else hipLaunchKernelGGL(norm_join_kernel<RT_F16>, grid, dim3(256), 0, v.stream, k, first);
+        if (a.dtype == RT_F32) hipLaunchKernelGGL(norm_join_kernel<RT_F32>, grid, dim3(1024), 0, v.stream, k, first);
+        else if (a.dtype == RT_BF16) hipLaunchKernelGGL(norm_join_kernel<RT_BF16>, grid, dim3(1024), 0, v.stream, k, first);
+        else hipLaunchKernelGGL(norm_join_kernel<RT_F16>, grid, dim3(1024), 0, v.stream, k, first);
         HIPCHK(ctx, hipGetLastError());
     }
     return RT_OK;

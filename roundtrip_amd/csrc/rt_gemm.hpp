@@ -364,20 +364,31 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
     }
 }
 
-// Joins the partial sums of the K splits, in their order, and finishes them.
+// Joins the partial sums of the K splits, in their order, and finishes them.  Eight splits' loads are under way at a time:
+// they come from other XCDs' writes, about a microsecond each.
 template <int DT, int EPI>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
+    constexpr int DUAL = EPI == EPI_GATED ? 2 : 1, B = 8 / DUAL;
     const int quads = a.Np >> 2, z = blockIdx.z;
     const long long total = a.M * quads, slot = a.M * a.Np;
-    for (long long p = (long long)blockIdx.x * 256 + threadIdx.x; p < total; p += (long long)gridDim.x * 256) {
+    for (long long p = (long long)blockIdx.x * blockDim.x + threadIdx.x; p < total; p += (long long)gridDim.x * blockDim.x) {
         const long long m = p / quads;
         const int n = (int)(p - m * quads) * 4;
         const float* q = a.part + (long long)z * slot + m * a.Np + n;
-        f32x4 v0 = {0, 0, 0, 0}, v1 = {0, 0, 0, 0};
-        for (int s = 0; s < a.splits; ++s) {
-            v0 += *(const f32x4*)(q + (long long)s * a.nslot * slot);
-            if (EPI == EPI_GATED) v1 += *(const f32x4*)(q + ((long long)s * a.nslot + 1) * slot);
+        f32x4 v[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        for (int s = 0; s < a.splits; s += B) {
+            f32x4 t[B][DUAL];
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int d = 0; d < DUAL; ++d)
+                    t[b][d] = *(const f32x4*)(q + ((long long)(s + b < a.splits ? s + b : s) * a.nslot + d) * slot);
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int d = 0; d < DUAL; ++d)
+                    if (s + b < a.splits) v[d] += t[b][d];
         }
-        epilogue<DT, EPI>(a, z, m, n, v0, v1);
+        epilogue<DT, EPI>(a, z, m, n, v[0], v[1]);
     }
 }

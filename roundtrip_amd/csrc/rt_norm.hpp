@@ -4,7 +4,8 @@
 //   N(v; w) = v' / sqrt(mean(v'^2) + eps) * (w + w_offset),   v' = v (rms) or v - mean(v) (layer)
 //
 // Bound by memory: a row is read once and held in registers (TPR threads a row, NV 16-byte chunks a thread) while its
-// sums are made in float32, and every output is written once.
+// sums are made in float32, and every output is written once.  What limits short calls is the chain load - sum - load: all
+// of a row's arrays are asked for before the first is used, and sums that do not wait for each other share one exchange.
 #pragma once
 #include "rt_elem.hpp"
 
@@ -22,163 +23,158 @@ struct NormArgs {
     long long lddy, lddn, lddx, lddb, lddg;
     float yin_scale;                                 // y = yin_scale * yin
     int want_post, want_pre;
-    long long rows_per_unit;                         // consecutive rows of one unit (TPR threads)
+    long long rows_per_unit;                         // consecutive rows of one workgroup
     int units;
+    int together;                                    // the waves of a workgroup share its rows' gate sums
     float *p_post, *p_pre, *p_gate;                  // [units][d], [units][d], [units][2][d] partial sums
     char *dw_post, *dw_pre;
 };
 
-// Sum over the TPR threads of a row, the same value in all of them.  sm: one float a wave, two sets used in turn.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* sm, int& turn) {
+// K sums over the TPR threads of a row, the same values in all of them.  sm: K floats a wave, two sets used in turn, so that
+// one barrier a call is enough.
+template <int TPR, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float (*sm)[4], int& turn) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o, 64);
     if (TPR > 64) {
         constexpr int W = TPR / 64;
-        float* s = sm + (turn & 1) * W;
+        float(*s)[4] = sm + (turn & 1) * W;
         turn++;
         const int wave = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) s[wave] = v;
-        __syncthreads();
-        v = 0.0f;
+        if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) v += s[w];
+            for (int k = 0; k < K; ++k) s[wave][k] = v[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+#pragma unroll
+            for (int k = 0; k < K; ++k) v[k] += s[w][k];
     }
-    return v;
 }
 
-// A row in registers, in float32.  hat(): v -> (v - mean) r, returns r.
+#define FOR_ROW(k, e)                        \
+    _Pragma("unroll") for (int k = 0; k < NV; ++k) _Pragma("unroll") for (int e = 0; e < E; ++e)
+
+// A row as it lies in memory.
+template <int DT, int TPR, int NV, bool AL>
+struct Raw {
+    static constexpr int E = EPC<DT>;
+    u32x4 c[NV];
+    __device__ __forceinline__ void load(const char* p, int d, int t) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int at = (k * TPR + t) * E;
+            c[k] = u32x4{0, 0, 0, 0};
+            if (at < d) c[k] = load_chunk<DT, AL>(p + (long long)at * ES<DT>, d - at);
+        }
+    }
+};
+
+// A row in registers, in float32.
 template <int DT, int TPR, int NV, bool AL>
 struct Row {
     static constexpr int E = EPC<DT>;
     float v[NV][E];
 
-    __device__ __forceinline__ void load(const char* p, int d, int t) {
+    __device__ __forceinline__ Row() {}
+    __device__ __forceinline__ explicit Row(const Raw<DT, TPR, NV, AL>& r) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * TPR + t) * E;
-            u32x4 q = {0, 0, 0, 0};
-            if (c < d) q = load_chunk<DT, AL>(p + (long long)c * ES<DT>, d - c);
-            chunk_to_f32<DT>(q, v[k]);
-        }
+        for (int k = 0; k < NV; ++k) chunk_to_f32<DT>(r.c[k], v[k]);
+    }
+    // a weight: ones where there is none
+    __device__ __forceinline__ Row(const Raw<DT, TPR, NV, AL>& r, const char* p, float off) : Row(r) {
+        FOR_ROW(k, e) v[k][e] = p ? v[k][e] + off : 1.0f;
     }
     __device__ __forceinline__ void store(char* p, int d, int t) const {
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = (k * TPR + t) * E;
-            if (c < d) store_chunk<DT, AL>(p + (long long)c * ES<DT>, v[k], d - c);
+            const int at = (k * TPR + t) * E;
+            if (at < d) store_chunk<DT, AL>(p + (long long)at * ES<DT>, v[k], d - at);
         }
     }
-    __device__ __forceinline__ float hat(int d, int t, int kind, float eps, float* sm, int& turn) {
-        const float inv = 1.0f / (float)d;
-        if (kind == RT_NORM_LAYER) {
-            float s = 0.0f;
+    __device__ __forceinline__ void put(float* p, int d, int t) const {
 #pragma unroll
-            for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+            const int at = (k * TPR + t) * E;
 #pragma unroll
-                for (int e = 0; e < E; ++e) s += v[k][e];
-            const float mean = row_sum<TPR>(s, sm, turn) * inv;
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[k][e] = (k * TPR + t) * E + e < d ? v[k][e] - mean : 0.0f;
+            for (int e = 0; e < E; ++e)
+                if (at + e < d) p[at + e] = v[k][e];
         }
-        float q = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) q += v[k][e] * v[k][e];
-        const float r = 1.0f / sqrtf(row_sum<TPR>(q, sm, turn) * inv + eps);
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[k][e] *= r;
-        return r;
     }
-    // the gradient through hat: this holds the hatted row, z the gradient of it, r its factor; z becomes the result
-    __device__ __forceinline__ void back(Row& z, int d, int t, int kind, float r, float* sm, int& turn) const {
-        const float inv = 1.0f / (float)d;
-        float p = 0.0f, s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const bool in = (k * TPR + t) * E + (AL ? 0 : e) < d;        // nothing behind the row's end counts
-                p += in ? z.v[k][e] * v[k][e] : 0.0f;
-                s += in ? z.v[k][e] : 0.0f;
-            }
-        p = row_sum<TPR>(p, sm, turn) * inv;
-        s = kind == RT_NORM_LAYER ? row_sum<TPR>(s, sm, turn) * inv : 0.0f;      // the hatted row sums to 0
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) z.v[k][e] = (z.v[k][e] - v[k][e] * p - s) * r;
+    __device__ __forceinline__ void zero() { FOR_ROW(k, e) v[k][e] = 0.0f; }
+    __device__ __forceinline__ float sum() const {
+        float s = 0.0f;
+        FOR_ROW(k, e) s += v[k][e];
+        return s;
     }
+    __device__ __forceinline__ float dot(const Row& o) const {
+        float s = 0.0f;
+        FOR_ROW(k, e) s += v[k][e] * o.v[k][e];
+        return s;
+    }
+    // v - mean, and zeros behind the row's end
+    __device__ __forceinline__ void centre(float mean, int d, int t) {
+        FOR_ROW(k, e) v[k][e] = (k * TPR + t) * E + (AL ? 0 : e) < d ? v[k][e] - mean : 0.0f;
+    }
+    __device__ __forceinline__ void scale(float f) { FOR_ROW(k, e) v[k][e] *= f; }
 };
-
-template <int DT, int TPR, int NV, bool AL>
-__device__ __forceinline__ void load_weight(Row<DT, TPR, NV, AL>& w, const char* p, float off, int d, int t) {
-    if (p) {
-        w.load(p, d, t);
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < EPC<DT>; ++e) w.v[k][e] += off;
-    } else {
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < EPC<DT>; ++e) w.v[k][e] = 1.0f;
-    }
-}
 
 constexpr int norm_block(int TPR) { return TPR > 256 ? TPR : 256; }
 
 template <int DT, int TPR, int NV, bool AL>
 __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
     typedef Row<DT, TPR, NV, AL> R;
+    typedef Raw<DT, TPR, NV, AL> M;
     constexpr int E = EPC<DT>;
-    __shared__ float sm[2 * (TPR > 64 ? TPR / 64 : 1)];
+    __shared__ float sm[2 * (TPR > 64 ? TPR / 64 : 1)][4];
     int turn = 0;
     const int t = threadIdx.x % TPR;
     const long long row = (long long)blockIdx.x * (norm_block(TPR) / TPR) + threadIdx.x / TPR;
     if (row >= a.T) return;                     // TPR > 64: the whole workgroup (one row); else the whole wave
-    R v;
-    v.load(a.x + row * a.ldx, a.d, t);
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < E; ++e) v.v[k][e] *= a.rs;
+    const float inv = 1.0f / (float)a.d;
+    M mx, mb, mg, mpost = {}, mpre = {};
+    mx.load(a.x + row * a.ldx, a.d, t);
+    if (a.b) mb.load(a.b + row * a.ldb, a.d, t);
+    if (a.b && a.gate) mg.load(a.gate + (row / a.rpg) * a.ldg, a.d, t);
+    if (a.b && a.w_post) mpost.load(a.w_post, a.d, t);
+    if (a.n && a.w_pre) mpre.load(a.w_pre, a.d, t);
+    R v(mx);
+    v.scale(a.rs);
     if (a.b) {
-        R b, w;
-        b.load(a.b + row * a.ldb, a.d, t);
-        b.hat(a.d, t, a.kind, a.eps, sm, turn);
-        load_weight(w, a.w_post, a.w_off, a.d, t);
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) b.v[k][e] *= w.v[k][e] * a.bs;
-        if (a.gate) {
-            w.load(a.gate + (row / a.rpg) * a.ldg, a.d, t);
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) b.v[k][e] *= w.v[k][e];
+        R b(mb), w(mpost, a.w_post, a.w_off);
+        float s[1];
+        if (a.kind == RT_NORM_LAYER) {
+            s[0] = b.sum();
+            row_sums<TPR>(s, sm, turn);
+            b.centre(s[0] * inv, a.d, t);
         }
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v.v[k][e] += b.v[k][e];
+        s[0] = b.dot(b);
+        row_sums<TPR>(s, sm, turn);
+        const float f = 1.0f / sqrtf(s[0] * inv + a.eps) * a.bs;
+        if (a.gate) {
+            R g(mg);
+            FOR_ROW(k, e) w.v[k][e] *= g.v[k][e];
+        }
+        FOR_ROW(k, e) v.v[k][e] += b.v[k][e] * f * w.v[k][e];
     }
     if (a.y) v.store(a.y + row * a.ldy, a.d, t);
     if (a.n) {
-        R w;
-        v.hat(a.d, t, a.kind, a.eps, sm, turn);
-        load_weight(w, a.w_pre, a.w_off, a.d, t);
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v.v[k][e] *= w.v[k][e];
+        float s[1];
+        if (a.kind == RT_NORM_LAYER) {
+            s[0] = v.sum();
+            row_sums<TPR>(s, sm, turn);
+            v.centre(s[0] * inv, a.d, t);
+        }
+        s[0] = v.dot(v);
+        row_sums<TPR>(s, sm, turn);
+        const float f = 1.0f / sqrtf(s[0] * inv + a.eps);
+        R w(mpre, a.w_pre, a.w_off);
+        FOR_ROW(k, e) v.v[k][e] *= f * w.v[k][e];
         v.store(a.n + row * a.ldn, a.d, t);
     }
 }
@@ -188,152 +184,218 @@ __device__ __forceinline__ int gate_slot(long long group, long long unit_row0, l
     return group * rpg <= unit_row0 ? 0 : 1;
 }
 
-// A unit (TPR threads) walks rows_per_unit consecutive rows and holds its column sums in registers; a gate's sum is
-// written when its rows end: to dgate if the unit saw all of them, else to one of the unit's two partial slots.
+// Backward.  A unit is a workgroup: it walks rows_per_unit consecutive rows, all its threads one row at a time (TPR > 64) or a
+// row for each of its four waves (TPR = 64), and its threads hold the column sums; a row's arrays are loaded while the row
+// before is worked on.  The rows of one gate are a segment.  Where segments are long, the waves take its rows in turn
+// (`together`) and their sums meet in LDS at its end; where short, a wave takes whole segments.  A segment's sum goes to
+// dgate if the unit saw all of the gate's rows, else to one of the unit's two partial slots.
+//
+//   t = dy + dN(dn w_pre at y);  dx = rs t;  q = bs t;  db = dN(q gate w_post at b)
+//   dN(z at v) = r (z - vh mean(z vh) [- mean z]),  vh = r v',  r = 1 / sqrt(mean(v'^2) + eps)
 template <int DT, int TPR, int NV, bool AL>
 __global__ __launch_bounds__(norm_block(TPR)) void norm_back_kernel(NormArgs a) {
     typedef Row<DT, TPR, NV, AL> R;
-    constexpr int E = EPC<DT>;
-    __shared__ float sm[2 * (TPR > 64 ? TPR / 64 : 1)];
+    typedef Raw<DT, TPR, NV, AL> M;
+    constexpr int E = EPC<DT>, WAVES = norm_block(TPR) / TPR, COLS = TPR * NV * E;
+    __shared__ float sm[2 * (TPR > 64 ? TPR / 64 : 1)][4];
+    __shared__ float meet[WAVES > 1 ? WAVES * COLS : 1];
     int turn = 0;
-    const int t = threadIdx.x % TPR, unit = blockIdx.x * (norm_block(TPR) / TPR) + threadIdx.x / TPR;
+    const int t = threadIdx.x % TPR, w = threadIdx.x / TPR, unit = blockIdx.x;
     const long long r0 = unit * a.rows_per_unit, r1 = r0 + a.rows_per_unit < a.T ? r0 + a.rows_per_unit : a.T;
-    if (r0 >= r1) return;
-    float s_post[NV][E], s_pre[NV][E], s_gate[NV][E];
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int e = 0; e < E; ++e) s_post[k][e] = s_pre[k][e] = s_gate[k][e] = 0.0f;
+    const float inv = 1.0f / (float)a.d;
+    const bool layer = a.kind == RT_NORM_LAYER;
+    M mpost = {}, mpre = {};
+    if (a.b && a.w_post) mpost.load(a.w_post, a.d, t);
+    if (a.dn && a.w_pre) mpre.load(a.w_pre, a.d, t);
 
-    auto put = [&](float* p, float (&s)[NV][E]) {
+    R s_post, s_pre, s_gate;
+    s_post.zero();
+    s_pre.zero();
+    s_gate.zero();
+
+    // the waves' sums, added in wave order, in wave 0
+    auto join = [&](R& s) __attribute__((always_inline)) {
+        if (WAVES > 1) {
+            __syncthreads();
+            if (w) s.put(meet + w * COLS, a.d, t);
+            __syncthreads();
+            if (w == 0) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * TPR + t) * E;
+                for (int k = 0; k < NV; ++k) {
+                    const int at = (k * TPR + t) * E;
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (c + e < a.d) p[c + e] = s[k][e];
+                    for (int e = 0; e < E; ++e)
+                        if (at + e < a.d)
+#pragma unroll
+                            for (int o = 1; o < WAVES; ++o) s.v[k][e] += meet[o * COLS + at + e];
+                }
+            }
+        }
+    };
+    auto flush = [&](long long group) __attribute__((always_inline)) {       // the segment of this gate is done
+        const long long g0 = group * a.rpg, g1 = g0 + a.rpg < a.T ? g0 + a.rpg : a.T;
+        if (g0 >= r0 && g1 <= r1) s_gate.store(a.dgate + group * a.lddg, a.d, t);
+        else s_gate.put(a.p_gate + ((long long)unit * 2 + gate_slot(group, r0, a.rpg)) * a.d, a.d, t);
+    };
+
+    struct Arrays {
+        M y, dn, dy, b, g;
+    } cur, nxt;
+    auto fetch = [&](Arrays& m, long long row) __attribute__((always_inline)) {
+        if (a.dn) {
+            m.y.load(a.yin + row * a.ldy, a.d, t);
+            m.dn.load(a.dn + row * a.lddn, a.d, t);
+        }
+        if (a.dy) m.dy.load(a.dy + row * a.lddy, a.d, t);
+        if (a.b) m.b.load(a.b + row * a.ldb, a.d, t);
+        if (a.gate) m.g.load(a.gate + (row / a.rpg) * a.ldg, a.d, t);
+    };
+    auto work = [&](const Arrays& m, long long row) __attribute__((always_inline)) {
+        R z, y, b;
+        float first[4] = {0, 0, 0, 0};             // means of y and of b, then of y^2, z y, z and b^2
+        if (a.b) b = R(m.b);
+        if (a.dn) {
+            y = R(m.y);
+            y.scale(a.yin_scale);
+            z = R(m.dn);
+        }
+        if (layer) {
+            float s[2] = {a.dn ? y.sum() : 0.0f, a.b ? b.sum() : 0.0f};
+            row_sums<TPR>(s, sm, turn);
+            if (a.dn) y.centre(s[0] * inv, a.d, t);
+            if (a.b) b.centre(s[1] * inv, a.d, t);
+        }
+        R dn;
+        if (a.dn) {
+            dn = z;
+            const R wp(mpre, a.w_pre, a.w_off);
+            FOR_ROW(k, e) z.v[k][e] *= wp.v[k][e];
+            first[0] = y.dot(y);
+            first[1] = z.dot(y);
+            first[2] = layer ? z.sum() : 0.0f;     // nothing lies behind the row's end: dn is 0 there
+        }
+        if (a.b) first[3] = b.dot(b);
+        row_sums<TPR>(first, sm, turn);
+        if (a.dn) {
+            const float r = 1.0f / sqrtf(first[0] * inv + a.eps), p = r * first[1] * inv, q = first[2] * inv;
+            FOR_ROW(k, e) {
+                const float h = y.v[k][e] * r;
+                s_pre.v[k][e] += dn.v[k][e] * h;
+                z.v[k][e] = (z.v[k][e] - h * p - q) * r;
+            }
+        }
+        if (a.dy) {
+            const R dy(m.dy);
+            FOR_ROW(k, e) z.v[k][e] = a.dn ? z.v[k][e] + dy.v[k][e] : dy.v[k][e];
+        }
+        if (a.dx) {
+            R dx;
+            FOR_ROW(k, e) dx.v[k][e] = z.v[k][e] * a.rs;
+            dx.store(a.dx + row * a.lddx, a.d, t);
+        }
+        if (!a.b) return;
+        const float r = 1.0f / sqrtf(first[3] * inv + a.eps);
+        const R wp(mpost, a.w_post, a.w_off), g(m.g);
+        FOR_ROW(k, e) {
+            const float q = z.v[k][e] * a.bs, gt = a.gate ? g.v[k][e] : 1.0f;
+            b.v[k][e] *= r;
+            s_gate.v[k][e] += q * b.v[k][e] * wp.v[k][e];
+            s_post.v[k][e] += q * gt * b.v[k][e];
+            z.v[k][e] = (k * TPR + t) * E + (AL ? 0 : e) < a.d ? q * gt * wp.v[k][e] : 0.0f;
+        }
+        if (a.db) {
+            float s[2] = {z.dot(b), layer ? z.sum() : 0.0f};
+            row_sums<TPR>(s, sm, turn);
+            FOR_ROW(k, e) z.v[k][e] = (z.v[k][e] - b.v[k][e] * (s[0] * inv) - s[1] * inv) * r;
+            z.store(a.db + row * a.lddb, a.d, t);
         }
     };
 
-    for (long long row = r0; row < r1; ++row) {
-        R z, h;
-        // t = dy + the gradient through n = N(y)
-        if (a.dn) {
-            R y, w;
-            y.load(a.yin + row * a.ldy, a.d, t);
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) y.v[k][e] *= a.yin_scale;
-            const float r = y.hat(a.d, t, a.kind, a.eps, sm, turn);
-            z.load(a.dn + row * a.lddn, a.d, t);
-            load_weight(w, a.w_pre, a.w_off, a.d, t);
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    s_pre[k][e] += z.v[k][e] * y.v[k][e];
-                    z.v[k][e] *= w.v[k][e];
-                }
-            y.back(z, a.d, t, a.kind, r, sm, turn);
-            if (a.dy) {
-                h.load(a.dy + row * a.lddy, a.d, t);
-#pragma unroll
-                for (int k = 0; k < NV; ++k)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) z.v[k][e] += h.v[k][e];
+    // rows first, first + step, .. < end
+    auto walk = [&](long long first, long long end, long long step, bool own_segments) __attribute__((always_inline)) {
+        if (first < end) fetch(cur, first);
+        for (long long row = first; row < end; row += step) {
+            if (row + step < end) fetch(nxt, row + step);
+            work(cur, row);
+            if (own_segments && a.dgate && (row + 1 == end || (row + 1) % a.rpg == 0)) {
+                flush(row / a.rpg);
+                s_gate.zero();
             }
-        } else {
-            z.load(a.dy + row * a.lddy, a.d, t);
+            cur = nxt;
         }
-        if (a.dx) {
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) h.v[k][e] = z.v[k][e] * a.rs;
-            h.store(a.dx + row * a.lddx, a.d, t);
-        }
-        if (!a.b) continue;
-        R w, gt;
-        h.load(a.b + row * a.ldb, a.d, t);
-        const float r = h.hat(a.d, t, a.kind, a.eps, sm, turn);
-        load_weight(w, a.w_post, a.w_off, a.d, t);
-        const long long group = row / a.rpg;
-        if (a.gate) {
-            gt.load(a.gate + group * a.ldg, a.d, t);
-        } else {
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) gt.v[k][e] = 1.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < NV; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float q = z.v[k][e] * a.bs;
-                s_gate[k][e] += q * h.v[k][e] * w.v[k][e];
-                s_post[k][e] += q * gt.v[k][e] * h.v[k][e];
-                z.v[k][e] = q * gt.v[k][e] * w.v[k][e];
+    };
+
+    // (by the gate, not by whether its gradient is wanted: the other sums keep their order)
+    if (!a.gate) {
+        walk(r0 + w, r1, WAVES, false);
+    } else if (WAVES == 1 || !a.together) {
+        // whole segments to a wave: its share of the unit's segments, in a row
+        const long long n = WAVES > 1 ? (a.rows_per_unit / a.rpg + WAVES - 1) / WAVES * a.rpg : a.rows_per_unit;
+        const long long b0 = r0 + w * n, b1 = b0 + n < r1 ? b0 + n : r1;
+        walk(b0, b1, 1, true);
+    } else {
+        for (long long s0 = r0; s0 < r1;) {
+            const long long group = s0 / a.rpg, s1 = (group + 1) * a.rpg < r1 ? (group + 1) * a.rpg : r1;
+            walk(s0 + w, s1, WAVES, false);
+            if (a.dgate) {
+                join(s_gate);
+                if (w == 0) flush(group);
+                s_gate.zero();
             }
-        if (a.db) {
-            h.back(z, a.d, t, a.kind, r, sm, turn);
-            z.store(a.db + row * a.lddb, a.d, t);
-        }
-        if (a.dgate && (row + 1 == r1 || (row + 1) % a.rpg == 0)) {
-            const long long g0 = group * a.rpg, g1 = g0 + a.rpg < a.T ? g0 + a.rpg : a.T;
-            if (g0 >= r0 && g1 <= r1) {
-#pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    const int c = (k * TPR + t) * E;
-                    if (c < a.d) store_chunk<DT, AL>(a.dgate + group * a.lddg + (long long)c * ES<DT>, s_gate[k], a.d - c);
-                }
-            } else {
-                put(a.p_gate + ((long long)unit * 2 + gate_slot(group, r0, a.rpg)) * a.d, s_gate);
-            }
-#pragma unroll
-            for (int k = 0; k < NV; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) s_gate[k][e] = 0.0f;
+            s0 = s1;
         }
     }
-    if (a.want_post) put(a.p_post + (long long)unit * a.d, s_post);
-    if (a.want_pre) put(a.p_pre + (long long)unit * a.d, s_pre);
+    if (a.want_post) {
+        join(s_post);
+        if (w == 0) s_post.put(a.p_post + (long long)unit * a.d, a.d, t);
+    }
+    if (a.want_pre) {
+        join(s_pre);
+        if (w == 0) s_pre.put(a.p_pre + (long long)unit * a.d, a.d, t);
+    }
 }
 
-// Column sums of the units' partial sums, in a fixed order: 32 columns x 8 row classes a workgroup.
+// Column sums of the units' partial sums, in a fixed order: 32 columns x 32 row classes a workgroup, eight rows of a class under
+// way at a time.
 // blockIdx.y + first: 0 post, 1 pre, 2 + g: gate group g (of those, only what more than one unit saw).
 template <int DT>
-__global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, int first) {
+__global__ __launch_bounds__(1024) void norm_join_kernel(NormArgs a, int first) {
     typedef typename Elem<DT>::T T;
-    __shared__ float sm[8][33];
+    constexpr int RC = 32, B = 8;
+    __shared__ float sm[RC][33];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), rc = threadIdx.x >> 5, what = blockIdx.y + first;
-    const float* p;
-    char* out;
+    const long long group = what - 2;
+    const float* p = what == 0 ? a.p_post : a.p_pre;
+    char* out = what == 0 ? a.dw_post : a.dw_pre;
     long long u0 = 0, u1 = a.units;
-    if (what < 2) {
-        p = what == 0 ? a.p_post : a.p_pre;
-        out = what == 0 ? a.dw_post : a.dw_pre;
-        if (!out) return;
-    } else {
-        const long long g = what - 2, g0 = g * a.rpg, g1 = g0 + a.rpg < a.T ? g0 + a.rpg : a.T;
+    if (what >= 2) {
+        const long long g0 = group * a.rpg, g1 = g0 + a.rpg < a.T ? g0 + a.rpg : a.T;
         u0 = g0 / a.rows_per_unit;
         u1 = (g1 - 1) / a.rows_per_unit + 1;
         if (u1 - u0 == 1) return;
-        p = nullptr;
-        out = a.dgate + g * a.lddg;
+        out = a.dgate + group * a.lddg;
     }
+    if (!out) return;
     float s = 0.0f;
     if (c < a.d)
-        for (long long u = u0 + rc; u < u1; u += 8)
-            s += what < 2 ? p[u * a.d + c]
-                          : a.p_gate[(u * 2 + gate_slot(what - 2, u * a.rows_per_unit, a.rpg)) * a.d + c];
+        for (long long u = u0 + rc; u < u1; u += RC * B) {
+            float v[B];
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                const long long at = u + b * RC;
+                v[b] = 0.0f;
+                if (at < u1)
+                    v[b] = what < 2 ? p[at * a.d + c] : a.p_gate[(at * 2 + gate_slot(group, at * a.rows_per_unit, a.rpg)) * a.d + c];
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b) s += v[b];
+        }
     sm[rc][threadIdx.x & 31] = s;
     __syncthreads();
     if (rc == 0 && c < a.d) {
         float v = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v += sm[k][threadIdx.x & 31];
+        for (int k = 0; k < RC; ++k) v += sm[k][threadIdx.x & 31];
         ((T*)out)[c] = (T)v;
     }
 }
