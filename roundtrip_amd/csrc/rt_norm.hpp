@@ -30,14 +30,27 @@ struct NormArgs {
     char *dw_post, *dw_pre;
 };
 
+// A wave's sum in all its lanes, the same bits in each: within sixteen lanes by data-parallel moves, then across the rows of
+// sixteen.  (ds_bpermute takes ten times as long a step, and a row waits for three such sums.)
+__device__ __forceinline__ float wave_sum(float v) {
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, true));     // lane ^ 1
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, true));     // lane ^ 2
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xf, 0xf, true));    // 7 - lane
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xf, 0xf, true));    // 15 - lane
+    auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned a0 = a[0], a1 = a[1];
+    v = __builtin_bit_cast(float, a0) + __builtin_bit_cast(float, a1);
+    auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned b0 = b[0], b1 = b[1];
+    return __builtin_bit_cast(float, b0) + __builtin_bit_cast(float, b1);
+}
+
 // K sums over the TPR threads of a row, the same values in all of them.  sm: K floats a wave, two sets used in turn, so that
 // one barrier a call is enough.
 template <int TPR, int K>
 __device__ __forceinline__ void row_sums(float (&v)[K], float (*sm)[4], int& turn) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o, 64);
+    for (int k = 0; k < K; ++k) v[k] = wave_sum(v[k]);
     if (TPR > 64) {
         constexpr int W = TPR / 64;
         float(*s)[4] = sm + (turn & 1) * W;
@@ -60,17 +73,29 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*sm)[4], int& tur
 #define FOR_ROW(k, e)                        \
     _Pragma("unroll") for (int k = 0; k < NV; ++k) _Pragma("unroll") for (int e = 0; e < E; ++e)
 
+// The buffer of one row: a row that is not there has no bytes, reads as zeros and drops what is written, so that loads and
+// stores need no branches around them and the compiler can count them.
+typedef __amdgpu_buffer_rsrc_t RowBuf;
+__device__ __forceinline__ RowBuf row_buf(const char* p, bool there, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, p && there ? bytes : 0, 0x00020000);
+}
+
 // A row as it lies in memory.
 template <int DT, int TPR, int NV, bool AL>
 struct Raw {
     static constexpr int E = EPC<DT>;
     u32x4 c[NV];
-    __device__ __forceinline__ void load(const char* p, int d, int t) {
+    __device__ __forceinline__ void load(const char* p, int d, int t, bool there = true) {
+        const RowBuf r = row_buf(p, there, d * ES<DT>);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int at = (k * TPR + t) * E;
-            c[k] = u32x4{0, 0, 0, 0};
-            if (at < d) c[k] = load_chunk<DT, AL>(p + (long long)at * ES<DT>, d - at);
+            if (AL) {
+                c[k] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at * ES<DT>, 0, 0));
+            } else {
+                c[k] = u32x4{0, 0, 0, 0};
+                if (p && there && at < d) c[k] = load_chunk<DT, AL>(p + (unsigned)at * (unsigned)ES<DT>, d - at);
+            }
         }
     }
 };
@@ -87,14 +112,30 @@ struct Row {
         for (int k = 0; k < NV; ++k) chunk_to_f32<DT>(r.c[k], v[k]);
     }
     // a weight: ones where there is none
-    __device__ __forceinline__ Row(const Raw<DT, TPR, NV, AL>& r, const char* p, float off) : Row(r) {
-        FOR_ROW(k, e) v[k][e] = p ? v[k][e] + off : 1.0f;
+    __device__ __forceinline__ void weight(const char* p, float off, int d, int t) {
+        if (p) {
+            Raw<DT, TPR, NV, AL> r;
+            r.load(p, d, t);
+            *this = Row(r);
+            FOR_ROW(k, e) v[k][e] += off;
+        } else {
+            FOR_ROW(k, e) v[k][e] = 1.0f;
+        }
     }
     __device__ __forceinline__ void store(char* p, int d, int t) const {
+        typedef typename Elem<DT>::T T;
+        const RowBuf r = row_buf(p, true, d * ES<DT>);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int at = (k * TPR + t) * E;
-            if (at < d) store_chunk<DT, AL>(p + (long long)at * ES<DT>, v[k], d - at);
+            if (AL) {
+                union { T t[E]; u32x4 c; } u;
+#pragma unroll
+                for (int e = 0; e < E; ++e) u.t[e] = (T)v[k][e];
+                __builtin_amdgcn_raw_buffer_store_b128(u.c, r, at * ES<DT>, 0, 0);
+            } else if (p && at < d) {
+                store_chunk<DT, AL>(p + (unsigned)at * (unsigned)ES<DT>, v[k], d - at);
+            }
         }
     }
     __device__ __forceinline__ void put(float* p, int d, int t) const {
@@ -121,6 +162,7 @@ struct Row {
     __device__ __forceinline__ void centre(float mean, int d, int t) {
         FOR_ROW(k, e) v[k][e] = (k * TPR + t) * E + (AL ? 0 : e) < d ? v[k][e] - mean : 0.0f;
     }
+    __device__ __forceinline__ void times(const Row& o, float off) { FOR_ROW(k, e) v[k][e] *= o.v[k][e] + off; }
     __device__ __forceinline__ void scale(float f) { FOR_ROW(k, e) v[k][e] *= f; }
 };
 
@@ -134,19 +176,21 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
     __shared__ float sm[2 * (TPR > 64 ? TPR / 64 : 1)][4];
     int turn = 0;
     const int t = threadIdx.x % TPR;
-    const long long row = (long long)blockIdx.x * (norm_block(TPR) / TPR) + threadIdx.x / TPR;
+    constexpr int WAVES = norm_block(TPR) / TPR;
+    const int w = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
+    const long long row = (long long)blockIdx.x * WAVES + w;
     if (row >= a.T) return;                     // TPR > 64: the whole workgroup (one row); else the whole wave
     const float inv = 1.0f / (float)a.d;
-    M mx, mb, mg, mpost = {}, mpre = {};
+    M mx, mb, mg, mpost, mpre;
     mx.load(a.x + row * a.ldx, a.d, t);
-    if (a.b) mb.load(a.b + row * a.ldb, a.d, t);
-    if (a.b && a.gate) mg.load(a.gate + (row / a.rpg) * a.ldg, a.d, t);
-    if (a.b && a.w_post) mpost.load(a.w_post, a.d, t);
-    if (a.n && a.w_pre) mpre.load(a.w_pre, a.d, t);
+    mb.load(a.b + row * a.ldb, a.d, t, a.b);
+    mg.load(a.gate + (long long)((unsigned)row / (unsigned)a.rpg) * a.ldg, a.d, t, a.gate);      // T < 2^31
+    mpost.load(a.w_post, a.d, t, a.b);
+    mpre.load(a.w_pre, a.d, t, a.n);
     R v(mx);
     v.scale(a.rs);
     if (a.b) {
-        R b(mb), w(mpost, a.w_post, a.w_off);
+        R b(mb);
         float s[1];
         if (a.kind == RT_NORM_LAYER) {
             s[0] = b.sum();
@@ -156,11 +200,10 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
         s[0] = b.dot(b);
         row_sums<TPR>(s, sm, turn);
         const float f = 1.0f / sqrtf(s[0] * inv + a.eps) * a.bs;
-        if (a.gate) {
-            R g(mg);
-            FOR_ROW(k, e) w.v[k][e] *= g.v[k][e];
-        }
-        FOR_ROW(k, e) v.v[k][e] += b.v[k][e] * f * w.v[k][e];
+        b.scale(f);
+        if (a.w_post) b.times(R(mpost), a.w_off);
+        if (a.gate) b.times(R(mg), 0.0f);
+        FOR_ROW(k, e) v.v[k][e] += b.v[k][e];
     }
     if (a.y) v.store(a.y + row * a.ldy, a.d, t);
     if (a.n) {
@@ -173,8 +216,8 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
         s[0] = v.dot(v);
         row_sums<TPR>(s, sm, turn);
         const float f = 1.0f / sqrtf(s[0] * inv + a.eps);
-        R w(mpre, a.w_pre, a.w_off);
-        FOR_ROW(k, e) v.v[k][e] *= f * w.v[k][e];
+        v.scale(f);
+        if (a.w_pre) v.times(R(mpre), a.w_off);
         v.store(a.n + row * a.ldn, a.d, t);
     }
 }
@@ -200,13 +243,14 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_back_kernel(NormArgs a) 
     __shared__ float sm[2 * (TPR > 64 ? TPR / 64 : 1)][4];
     __shared__ float meet[WAVES > 1 ? WAVES * COLS : 1];
     int turn = 0;
-    const int t = threadIdx.x % TPR, w = threadIdx.x / TPR, unit = blockIdx.x;
+    const int t = threadIdx.x % TPR, unit = blockIdx.x;
+    const int w = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);      // rows are the same for a whole wave
     const long long r0 = unit * a.rows_per_unit, r1 = r0 + a.rows_per_unit < a.T ? r0 + a.rows_per_unit : a.T;
     const float inv = 1.0f / (float)a.d;
     const bool layer = a.kind == RT_NORM_LAYER;
-    M mpost = {}, mpre = {};
-    if (a.b && a.w_post) mpost.load(a.w_post, a.d, t);
-    if (a.dn && a.w_pre) mpre.load(a.w_pre, a.d, t);
+    R w_post, w_pre;
+    w_post.weight(a.w_post, a.w_off, a.d, t);
+    w_pre.weight(a.w_pre, a.w_off, a.d, t);
 
     R s_post, s_pre, s_gate;
     s_post.zero();
@@ -240,53 +284,45 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_back_kernel(NormArgs a) 
 
     struct Arrays {
         M y, dn, dy, b, g;
-    } cur, nxt;
-    auto fetch = [&](Arrays& m, long long row) __attribute__((always_inline)) {
-        if (a.dn) {
-            m.y.load(a.yin + row * a.ldy, a.d, t);
-            m.dn.load(a.dn + row * a.lddn, a.d, t);
-        }
-        if (a.dy) m.dy.load(a.dy + row * a.lddy, a.d, t);
-        if (a.b) m.b.load(a.b + row * a.ldb, a.d, t);
-        if (a.gate) m.g.load(a.gate + (row / a.rpg) * a.ldg, a.d, t);
+    } even, odd;
+    auto fetch = [&](Arrays& m, long long row, long long group, bool there) __attribute__((always_inline)) {
+        m.y.load(a.yin + row * a.ldy, a.d, t, there && a.dn);
+        m.dn.load(a.dn + row * a.lddn, a.d, t, there && a.dn);
+        m.dy.load(a.dy + row * a.lddy, a.d, t, there && a.dy);
+        m.b.load(a.b + row * a.ldb, a.d, t, there && a.b);
+        m.g.load(a.gate + group * a.ldg, a.d, t, there && a.gate);
     };
     auto work = [&](const Arrays& m, long long row) __attribute__((always_inline)) {
-        R z, y, b;
-        float first[4] = {0, 0, 0, 0};             // means of y and of b, then of y^2, z y, z and b^2
-        if (a.b) b = R(m.b);
-        if (a.dn) {
-            y = R(m.y);
-            y.scale(a.yin_scale);
-            z = R(m.dn);
-        }
+        R y(m.y), dn(m.dn), b(m.b), z;
+        float sums[4] = {0, 0, 0, 0};              // of y^2, z y, z and b^2
+        if (a.yin_scale != 1.0f) y.scale(a.yin_scale);
         if (layer) {
-            float s[2] = {a.dn ? y.sum() : 0.0f, a.b ? b.sum() : 0.0f};
-            row_sums<TPR>(s, sm, turn);
-            if (a.dn) y.centre(s[0] * inv, a.d, t);
-            if (a.b) b.centre(s[1] * inv, a.d, t);
+            float mean[2] = {y.sum(), b.sum()};
+            row_sums<TPR>(mean, sm, turn);
+            y.centre(mean[0] * inv, a.d, t);
+            b.centre(mean[1] * inv, a.d, t);
         }
-        R dn;
         if (a.dn) {
-            dn = z;
-            const R wp(mpre, a.w_pre, a.w_off);
-            FOR_ROW(k, e) z.v[k][e] *= wp.v[k][e];
-            first[0] = y.dot(y);
-            first[1] = z.dot(y);
-            first[2] = layer ? z.sum() : 0.0f;     // nothing lies behind the row's end: dn is 0 there
+            FOR_ROW(k, e) z.v[k][e] = dn.v[k][e] * w_pre.v[k][e];
+            sums[0] = y.dot(y);
+            sums[1] = z.dot(y);
+            if (layer) sums[2] = z.sum();          // nothing lies behind the row's end: dn is 0 there
         }
-        if (a.b) first[3] = b.dot(b);
-        row_sums<TPR>(first, sm, turn);
+        if (a.b) sums[3] = b.dot(b);
+        row_sums<TPR>(sums, sm, turn);
         if (a.dn) {
-            const float r = 1.0f / sqrtf(first[0] * inv + a.eps), p = r * first[1] * inv, q = first[2] * inv;
+            const float r = 1.0f / sqrtf(sums[0] * inv + a.eps), p = r * sums[1] * inv, q = sums[2] * inv;
             FOR_ROW(k, e) {
                 const float h = y.v[k][e] * r;
                 s_pre.v[k][e] += dn.v[k][e] * h;
                 z.v[k][e] = (z.v[k][e] - h * p - q) * r;
             }
-        }
-        if (a.dy) {
-            const R dy(m.dy);
-            FOR_ROW(k, e) z.v[k][e] = a.dn ? z.v[k][e] + dy.v[k][e] : dy.v[k][e];
+            if (a.dy) {
+                const R dy(m.dy);
+                FOR_ROW(k, e) z.v[k][e] += dy.v[k][e];
+            }
+        } else {
+            z = R(m.dy);
         }
         if (a.dx) {
             R dx;
@@ -294,56 +330,79 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_back_kernel(NormArgs a) 
             dx.store(a.dx + row * a.lddx, a.d, t);
         }
         if (!a.b) return;
-        const float r = 1.0f / sqrtf(first[3] * inv + a.eps);
-        const R wp(mpost, a.w_post, a.w_off), g(m.g);
-        FOR_ROW(k, e) {
-            const float q = z.v[k][e] * a.bs, gt = a.gate ? g.v[k][e] : 1.0f;
-            b.v[k][e] *= r;
-            s_gate.v[k][e] += q * b.v[k][e] * wp.v[k][e];
-            s_post.v[k][e] += q * gt * b.v[k][e];
-            z.v[k][e] = (k * TPR + t) * E + (AL ? 0 : e) < a.d ? q * gt * wp.v[k][e] : 0.0f;
+        const float r = 1.0f / sqrtf(sums[3] * inv + a.eps);
+        b.scale(r);
+        z.scale(a.bs);
+        if (a.gate) {
+            const R g(m.g);
+            FOR_ROW(k, e) {
+                const float u = z.v[k][e] * b.v[k][e];
+                s_gate.v[k][e] += u * w_post.v[k][e];
+                s_post.v[k][e] += u * g.v[k][e];
+                z.v[k][e] *= g.v[k][e];
+            }
+        } else {
+            FOR_ROW(k, e) s_post.v[k][e] += z.v[k][e] * b.v[k][e];
         }
-        if (a.db) {
-            float s[2] = {z.dot(b), layer ? z.sum() : 0.0f};
-            row_sums<TPR>(s, sm, turn);
-            FOR_ROW(k, e) z.v[k][e] = (z.v[k][e] - b.v[k][e] * (s[0] * inv) - s[1] * inv) * r;
-            z.store(a.db + row * a.lddb, a.d, t);
+        if (!a.db) return;
+        FOR_ROW(k, e) z.v[k][e] *= w_post.v[k][e];
+        float last[2] = {z.dot(b), 0.0f};
+        if (layer) {
+            z.centre(0.0f, a.d, t);
+            last[1] = z.sum();
         }
+        row_sums<TPR>(last, sm, turn);
+        FOR_ROW(k, e) z.v[k][e] = (z.v[k][e] - b.v[k][e] * (last[0] * inv) - last[1] * inv) * r;
+        z.store(a.db + row * a.lddb, a.d, t);
     };
 
-    // rows first, first + step, .. < end
-    auto walk = [&](long long first, long long end, long long step, bool own_segments) __attribute__((always_inline)) {
-        if (first < end) fetch(cur, first);
-        for (long long row = first; row < end; row += step) {
-            if (row + step < end) fetch(nxt, row + step);
-            work(cur, row);
-            if (own_segments && a.dgate && (row + 1 == end || (row + 1) % a.rpg == 0)) {
-                flush(row / a.rpg);
+    // One segment after another (by the gate, not by whether its gradient is wanted: the other sums keep their order).
+    const bool own = a.gate && (WAVES == 1 || !a.together);         // a wave's rows are whole segments, in a row
+    for (long long s0 = r0; s0 < r1;) {
+        long long s1 = r1, row = s0 + w, end, step = WAVES;
+        if (WAVES > 1 && own) {
+            const unsigned n = ((unsigned)a.rows_per_unit / (unsigned)a.rpg + WAVES - 1) / WAVES * (unsigned)a.rpg;
+            row = r0 + (long long)w * n;
+            end = row + n < r1 ? row + n : r1;
+            step = 1;
+        }
+        // the row's gate and the row behind that gate's last: rows only go up, so it takes one division a segment (T < 2^31)
+        long long group = a.gate ? (unsigned)row / (unsigned)a.rpg : 0, g1 = (group + 1) * a.rpg;
+        if (!(WAVES > 1 && own)) {
+            if (a.gate && !own) {
+                const long long first = (long long)((unsigned)s0 / (unsigned)a.rpg) * a.rpg + a.rpg;
+                if (first < r1) s1 = first;
+            }
+            end = s1;
+        }
+        const long long seg_group = group;
+        fetch(even, row, group, row < end);
+        auto one = [&](const Arrays& now, Arrays& next) __attribute__((always_inline)) {
+            const bool ends = row + step >= end || row + step >= g1;      // of this gate's rows here
+            const long long here = group;
+            if (row + step >= g1) {
+                group++;
+                g1 += a.rpg;
+            }
+            fetch(next, row + step, group, row + step < end);
+            work(now, row);
+            if (own && a.dgate && ends) {
+                flush(here);
                 s_gate.zero();
             }
-            cur = nxt;
+            row += step;
+        };
+        while (row < end) {
+            one(even, odd);
+            if (row >= end) break;
+            one(odd, even);
         }
-    };
-
-    // (by the gate, not by whether its gradient is wanted: the other sums keep their order)
-    if (!a.gate) {
-        walk(r0 + w, r1, WAVES, false);
-    } else if (WAVES == 1 || !a.together) {
-        // whole segments to a wave: its share of the unit's segments, in a row
-        const long long n = WAVES > 1 ? (a.rows_per_unit / a.rpg + WAVES - 1) / WAVES * a.rpg : a.rows_per_unit;
-        const long long b0 = r0 + w * n, b1 = b0 + n < r1 ? b0 + n : r1;
-        walk(b0, b1, 1, true);
-    } else {
-        for (long long s0 = r0; s0 < r1;) {
-            const long long group = s0 / a.rpg, s1 = (group + 1) * a.rpg < r1 ? (group + 1) * a.rpg : r1;
-            walk(s0 + w, s1, WAVES, false);
-            if (a.dgate) {
-                join(s_gate);
-                if (w == 0) flush(group);
-                s_gate.zero();
-            }
-            s0 = s1;
+        if (a.gate && !own && a.dgate) {
+            join(s_gate);
+            if (w == 0) flush(seg_group);
+            s_gate.zero();
         }
+        s0 = s1;
     }
     if (a.want_post) {
         join(s_post);
