@@ -108,6 +108,7 @@ struct Product {                // C [M x N] = X W over K, nseg segments, nbatch
     int lx, lw, epi;
     int64_t M, K;
     int N, nseg, nbatch;
+    int nrun = nbatch;          // of the products side by side, how many are wanted: the plan, and so the bits, are the same
 };
 
 struct Plan {
@@ -144,10 +145,12 @@ void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
     pl.part_bytes = pl.splits > 1 ? (size_t)pl.splits * pl.nslot * p.M * pl.Np * sizeof(float) : 0;
 }
 
-int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, Plan& pl) {
+int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Plan& pl) {
     pl.skinny = false;
     const int ke = 128 / elem_size(dtype);
-    pl.bm = pl.bn = 128;
+    // 256 x 256 tiles where they fill the chip
+    const int64_t big = ((p.M + 255) / 256) * ((p.N + (p.epi == EPI_GATED ? 127 : 255)) / (p.epi == EPI_GATED ? 128 : 256)) * p.nbatch;
+    pl.bm = pl.bn = al && dtype != RT_F32 && big >= cus ? 256 : 128;
     const int cn = p.epi == EPI_GATED ? pl.bn / 2 : pl.bn;
     const int64_t tm = (p.M + pl.bm - 1) / pl.bm, tn = (p.N + cn - 1) / cn, nk = (p.K + ke - 1) / ke;
     if (tm * tn > 0x7fffffff || nk * p.nseg > 0x7fffffff)
@@ -202,9 +205,16 @@ int launch_product(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl
                         : p.lw == LI ? gemm_fn<DT, LK, LI, EPI_STORE>(al) : gemm_fn<DT, LK, LK, EPI_STORE>(al);
         join = gemm_join_kernel<DT, EPI_STORE>;
     }
-    hipLaunchKernelGGL(fn, dim3(pl.tiles_m * pl.tiles_n, pl.splits, p.nbatch), dim3(256), 0, st, a);
+    if constexpr (DT != RT_F32) {
+        if (pl.bm == 256)
+            fn = p.epi == EPI_GATED ? gemm_big_kernel<DT, LK, LI, EPI_GATED>
+                 : p.epi == EPI_GATED_BWD ? gemm_big_kernel<DT, LK, LK, EPI_GATED_BWD>
+                 : p.lx == LI ? gemm_big_kernel<DT, LI, LI, EPI_STORE>
+                 : p.lw == LI ? gemm_big_kernel<DT, LK, LI, EPI_STORE> : gemm_big_kernel<DT, LK, LK, EPI_STORE>;
+    }
+    hipLaunchKernelGGL(fn, dim3(pl.tiles_m * pl.tiles_n, pl.splits, p.nrun), dim3(pl.bm == 256 ? 512 : 256), 0, st, a);
     HIPCHK(ctx, hipGetLastError());
-    return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, p.nbatch, a) : RT_OK;
+    return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, p.nrun, a) : RT_OK;
 }
 
 template <int DT, int EPI, int MR>
@@ -234,9 +244,14 @@ int launch_skinny(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl,
 
 int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, GemmArgs& a) {
     Plan pl;
-    const int rc = plan_product(ctx, v.cu_count, dtype, p, pl);
-    if (rc) return rc;
     const int es = elem_size(dtype), epc = 16 / es;
+    a.quads = p.N % 4 == 0;
+    for (int i = 0; i < 3; ++i) {
+        const int os = p.epi == EPI_GATED && i ? 4 : es;      // what the forward pass keeps is float32
+        if (p.epi == EPI_STORE && i >= p.nrun) break;
+        a.quads = a.quads && (uintptr_t)a.o[i] % (4 * os) == 0 && a.ldo[i] % (4 * os) == 0;
+    }
+    if (p.epi == EPI_GATED_BWD) a.quads = a.quads && (uintptr_t)a.e[0] % 16 == 0 && (uintptr_t)a.e[1] % 16 == 0 && a.lde % 16 == 0;
     if (skinny_sizes(p) && a.ldw[0] % (4 * es) == 0 && (uintptr_t)a.w[0] % (4 * es) == 0 && (uintptr_t)a.w[1] % (4 * es) == 0) {
         plan_skinny(v.cu_count, dtype, p, pl);
         if (dtype == RT_F32) return launch_skinny<RT_F32>(ctx, v.stream, p, pl, a);
@@ -245,6 +260,8 @@ int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, Ge
     }
     bool al = (p.lx == LK ? p.K : p.M) % epc == 0 && (p.lw == LK ? p.K : p.N) % epc == 0 && a.ldx[0] % 16 == 0 && a.ldw[0] % 16 == 0;
     for (int i = 0; i < 2; ++i) al = al && (uintptr_t)a.x[i] % 16 == 0 && (uintptr_t)a.w[i] % 16 == 0;
+    const int rc = plan_product(ctx, v.cu_count, dtype, p, al, pl);
+    if (rc) return rc;
     if (dtype == RT_F32) return launch_product<RT_F32>(ctx, v.stream, p, pl, a, al);
     if (dtype == RT_BF16) return launch_product<RT_BF16>(ctx, v.stream, p, pl, a, al);
     return launch_product<RT_F16>(ctx, v.stream, p, pl, a, al);
@@ -271,11 +288,23 @@ struct Ffn {
     size_t h_bytes;
     Product gated, down;           // forward
     Product dh, dx, dw_in, dw_down;
-    Plan pl_gated, pl_down, pl_dh, pl_dx, pl_dw_in, pl_dw_down;
     size_t ws_fwd, ws_bwd;
 };
 
-size_t most(size_t a, size_t b) { return a > b ? a : b; }
+// Raises `most` to the bytes of partial sums this product can need.
+int most_part_bytes(rt_ctx* ctx, int cus, int dtype, const Product& p, size_t& most) {
+    Plan pl;
+    for (int al = 0; al < 2; ++al) {
+        const int rc = plan_product(ctx, cus, dtype, p, al, pl);
+        if (rc) return rc;
+        if (pl.part_bytes > most) most = pl.part_bytes;
+    }
+    if (skinny_sizes(p)) {
+        plan_skinny(cus, dtype, p, pl);
+        if (pl.part_bytes > most) most = pl.part_bytes;
+    }
+    return RT_OK;
+}
 
 int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& f) {
     if (!in) return failf(ctx, RT_EINVAL, "%s: the arguments are NULL", fn);
@@ -303,19 +332,15 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
     f.dw_down = {LI, LI, EPI_STORE, a.d_ff, a.T, a.d_out, 1, 1};
     f.ws_fwd = f.ws_bwd = 0;
     if (a.T == 0) return RT_OK;
+    // whichever kernels the call's alignment lets it use
+    size_t fwd = 0, bwd = 0;
     int rc;
-    if ((rc = plan_product(ctx, cus, a.dtype, f.gated, f.pl_gated)) || (rc = plan_product(ctx, cus, a.dtype, f.down, f.pl_down)) ||
-        (rc = plan_product(ctx, cus, a.dtype, f.dh, f.pl_dh)) || (rc = plan_product(ctx, cus, a.dtype, f.dx, f.pl_dx)) ||
-        (rc = plan_product(ctx, cus, a.dtype, f.dw_in, f.pl_dw_in)) || (rc = plan_product(ctx, cus, a.dtype, f.dw_down, f.pl_dw_down)))
-        return rc;
-    f.ws_fwd = f.h_bytes + most(f.pl_gated.part_bytes, f.pl_down.part_bytes);
     for (const Product* p : {&f.gated, &f.down})
-        if (skinny_sizes(*p)) {
-            Plan pl;
-            plan_skinny(cus, a.dtype, *p, pl);
-            f.ws_fwd = most(f.ws_fwd, f.h_bytes + pl.part_bytes);
-        }
-    f.ws_bwd = 3 * f.h_bytes + most(most(f.pl_dh.part_bytes, f.pl_dx.part_bytes), most(f.pl_dw_in.part_bytes, f.pl_dw_down.part_bytes));
+        if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, fwd))) return rc;
+    for (const Product* p : {&f.dh, &f.dx, &f.dw_in, &f.dw_down})
+        if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, bwd))) return rc;
+    f.ws_fwd = f.h_bytes + fwd;
+    f.ws_bwd = 3 * f.h_bytes + bwd;
     return RT_OK;
 }
 
@@ -388,7 +413,7 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
         set_w(g, r.dw_gate ? dg : du, r.dw_up ? du : dg, ldh);
         set_o(g, 0, r.dw_gate ? r.dw_gate : r.dw_up, r.ld_dw_in * es);
         set_o(g, 1, r.dw_up, r.ld_dw_in * es);
-        p.nbatch = r.dw_gate && r.dw_up ? 2 : 1;
+        p.nrun = r.dw_gate && r.dw_up ? 2 : 1;
         if ((rc = run_product(ctx, v, a.dtype, p, g))) return rc;
     }
     if (r.dw_down) {

@@ -25,11 +25,12 @@ struct GemmArgs {
     float* part;                   // splits > 1: [split][slot][M][Np] partial sums, joined by gemm_join_kernel
     int Np, nslot;
     char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two float32 or NULL).
-    long long ldo[3];              // EPI_GATED_BWD: dgate, dup, h
+    long long ldo[3];              // (EPI_STORE: ldo[0] for both)  EPI_GATED_BWD: dgate, dup, h
     const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept, float32
     long long lde;
     int act;
     float alpha;
+    int quads;                     // N and every output's (and e's) place are multiples of four elements
 };
 
 // ---- the gate's activation ----------------------------------------------------------------------------------------
@@ -42,66 +43,112 @@ __device__ __forceinline__ float sigmoid_f(float t) {
 }
 
 // a = act(g), d = act'(g).  gelu: the tanh form, 0.5 g (1 + tanh z) = g s(2z), which loses nothing where tanh z is near -1.
-template <int DT>
-__device__ __forceinline__ void act_f(int act, float alpha, float g, float& a, float& d) {
-    if (act == RT_ACT_LRELU) {
+template <int DT, int ACT>
+__device__ __forceinline__ void act_f(float alpha, float g, float& a, float& d) {
+    if (ACT == RT_ACT_LRELU) {
         d = g > 0.0f ? 1.0f : alpha;
         a = g * d;
-        return;
-    }
-    if (act == RT_ACT_GELU_TANH) {
+    } else if (ACT == RT_ACT_GELU_TANH) {
         const float c2 = 1.5957691216057308f, c3 = 0.044715f;      // 2 sqrt(2 / pi)
         const float s = sigmoid_f<DT>(c2 * (g + c3 * g * g * g));
         a = g * s;
         d = s + a * (1.0f - s) * c2 * (1.0f + 3.0f * c3 * g * g);
-        return;
+    } else {
+        const float s = sigmoid_f<DT>(g);
+        a = ACT == RT_ACT_SILU ? g * s : s;
+        d = ACT == RT_ACT_SILU ? s * (1.0f + g * (1.0f - s)) : s * (1.0f - s);
     }
-    const float s = sigmoid_f<DT>(g);
-    a = act == RT_ACT_SILU ? g * s : s;
-    d = act == RT_ACT_SILU ? s * (1.0f + g * (1.0f - s)) : s * (1.0f - s);
+}
+
+// Four values at p, of which `valid` exist; QUADS: all four do, and p is aligned to them.
+template <int DT, bool QUADS>
+__device__ __forceinline__ void put4(char* p, f32x4 v, int valid) {
+    typedef typename Elem<DT>::T T;
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (QUADS) *(T4*)p = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    else store4<DT>(p, v, valid);
 }
 
 // What becomes of four neighbouring sums of row m, columns n .. n+3 (v1: the second of EPI_GATED).
-template <int DT, int EPI>
+template <int DT, int EPI, int ACT, bool QUADS>
 __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, int n, f32x4 v0, f32x4 v1) {
     const int valid = a.N - n;
     if (valid <= 0) return;
-    const long long c = (long long)n * ES<DT>;
+    const long long c = (long long)n * ES<DT>, c4 = (long long)n * 4;
     if (EPI == EPI_STORE) {
-        store4<DT>(a.o[z] + m * a.ldo[z] + c, v0, valid);
+        put4<DT, QUADS>((z ? a.o[1] : a.o[0]) + m * a.ldo[0] + c, v0, valid);
     } else if (EPI == EPI_GATED) {
         f32x4 h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float t, d;
-            act_f<DT>(a.act, a.alpha, v0[j], t, d);
+            act_f<DT, ACT>(a.alpha, v0[j], t, d);
             h[j] = t * v1[j];
         }
-        store4<DT>(a.o[0] + m * a.ldo[0] + c, h, valid);
+        put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, h, valid);
         if (a.o[1]) {
-            store4<RT_F32>(a.o[1] + m * a.ldo[1] + n * 4ll, v0, valid);
-            store4<RT_F32>(a.o[2] + m * a.ldo[2] + n * 4ll, v1, valid);
+            put4<RT_F32, QUADS>(a.o[1] + m * a.ldo[1] + c4, v0, valid);
+            put4<RT_F32, QUADS>(a.o[2] + m * a.ldo[2] + c4, v1, valid);
         }
     } else {
-        const f32x4 g = load4<RT_F32>(a.e[0] + m * a.lde + n * 4ll, valid), u = load4<RT_F32>(a.e[1] + m * a.lde + n * 4ll, valid);
+        const char *pg = a.e[0] + m * a.lde + c4, *pu = a.e[1] + m * a.lde + c4;
+        const f32x4 g = QUADS ? *(const f32x4*)pg : load4<RT_F32>(pg, valid), u = QUADS ? *(const f32x4*)pu : load4<RT_F32>(pu, valid);
         f32x4 dg, du, h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float t, d;
-            act_f<DT>(a.act, a.alpha, g[j], t, d);
+            act_f<DT, ACT>(a.alpha, g[j], t, d);
             dg[j] = v0[j] * u[j] * d;
             du[j] = v0[j] * t;
             h[j] = t * u[j];
         }
-        store4<DT>(a.o[0] + m * a.ldo[0] + c, dg, valid);
-        store4<DT>(a.o[1] + m * a.ldo[1] + c, du, valid);
-        store4<DT>(a.o[2] + m * a.ldo[2] + c, h, valid);
+        put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, dg, valid);
+        put4<DT, QUADS>(a.o[1] + m * a.ldo[1] + c, du, valid);
+        put4<DT, QUADS>(a.o[2] + m * a.ldo[2] + c, h, valid);
+    }
+}
+
+// body(ACT, QUADS) with both as constants: the choice is made once, outside the loops over a tile.
+template <int ACT, bool QUADS> struct EpiWay {
+    static constexpr int act = ACT;
+    static constexpr bool quads = QUADS;
+};
+template <int EPI, class Body>
+__device__ __forceinline__ void epilogue_way(const GemmArgs& a, Body body) {
+    if (EPI == EPI_STORE) {
+        if (a.quads) body(EpiWay<0, true>());
+        else body(EpiWay<0, false>());
+    } else if (a.quads) {
+        if (a.act == RT_ACT_SILU) body(EpiWay<RT_ACT_SILU, true>());
+        else if (a.act == RT_ACT_GELU_TANH) body(EpiWay<RT_ACT_GELU_TANH, true>());
+        else if (a.act == RT_ACT_LRELU) body(EpiWay<RT_ACT_LRELU, true>());
+        else body(EpiWay<RT_ACT_SIGMOID, true>());
+    } else {
+        if (a.act == RT_ACT_SILU) body(EpiWay<RT_ACT_SILU, false>());
+        else if (a.act == RT_ACT_GELU_TANH) body(EpiWay<RT_ACT_GELU_TANH, false>());
+        else if (a.act == RT_ACT_LRELU) body(EpiWay<RT_ACT_LRELU, false>());
+        else body(EpiWay<RT_ACT_SIGMOID, false>());
     }
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// A buffer of `span` bytes from p on: what lies behind it reads as zeros.
+__device__ __forceinline__ u32x4 buffer_of(const char* p, int span) {
+    const unsigned long long at = (unsigned long long)p;
+    return u32x4{(unsigned)__builtin_amdgcn_readfirstlane((int)at), (unsigned)__builtin_amdgcn_readfirstlane((int)(at >> 32) & 0xffff),
+                 (unsigned)__builtin_amdgcn_readfirstlane(span), 0x00020000u};
+}
+
+// Sixteen bytes a lane straight to LDS, lane after lane from sm on (the same for the whole wave).  Written out because the
+// compiler, where it loses track of which of the two tiles a read of LDS belongs to, waits for all such loads before it;
+// whoever reads the tile waits for vmcnt(0) and a barrier.  (s_nop: m0 is set one wait state before its use.)
+__device__ __forceinline__ void load_to_lds(u32x4 r, char* sm, int off) {
+    const unsigned at = (unsigned)(uintptr_t)(lds_void*)sm;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(at), "v"(off), "s"(r) : "memory", "m0");
+}
 
 constexpr int OOB = 0x7fffff00;            // an offset that every buffer below ends before
 
@@ -177,7 +224,7 @@ struct Loader {
 #pragma unroll
             for (int it = 0; it < T::ITER; ++it) {
                 const bool second = L == LI && NSUB == 2 && it >= T::ITER / 2;
-                auto r = __builtin_amdgcn_make_buffer_rsrc((void*)((second ? base2 : base) + adv), 0, span, 0x00020000);
+                const u32x4 r = buffer_of((second ? base2 : base) + adv, span);
                 int v = voff[it];
                 if (L == LK && ke < T::KE) {            // the last tile: chunks behind K are zeros
                     int sub, idx, c;
@@ -189,7 +236,7 @@ struct Loader {
                     T::place(tid, it, sub, idx, c);
                     if (idx >= ke) v = OOB;
                 }
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(sm + (it * NT + wave * 64) * 16), 16, v, 0, 0, 0);
+                load_to_lds(r, sm + (it * NT + wave * 64) * 16, v);
             }
         } else {
 #pragma unroll
@@ -212,19 +259,17 @@ struct Loader {
     }
 };
 
-// Reads the fragment of sixteen rows (or columns) starting at 16 t, k step s (of two): lane (g = lane / 16, i = lane % 16)
+// Reads the fragment of sixteen rows (or columns) starting at 16 t of sub-tile `sub`, k step s (of two): lane (g = lane / 16, i = lane % 16)
 // gets row i, k = 32 s + 8 g .. + 7 (16-bit), 16 s + 4 g .. + 3 (float32).  The same k's for both operands is all that
 // the sum needs.
 template <int DT, int L, int R, int NSUB, int NT>
-__device__ __forceinline__ u32x4 read_frag(const char* sm, int lane, int t, int s) {
+__device__ __forceinline__ u32x4 read_frag(const char* sm, int lane, int sub, int t, int s) {
     typedef Tile<DT, L, R, NSUB, NT> T;
     const int i = lane & 15, g = lane >> 4;
     if (L == LK) {
         return *(const u32x4*)(sm + (16 * t + i) * 128 + (((4 * s + g) ^ (i >> 1)) << 4));
     } else {
-        constexpr int TS = T::SR / 16;                        // fragments of a sub-tile
-        sm += (t / TS) * (T::SUB_CHUNKS * 16);
-        t %= TS;
+        sm += sub * (T::SUB_CHUNKS * 16);
         if (ES<DT> == 4) {
             u32x4 r;
 #pragma unroll
@@ -267,6 +312,41 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int& tm
     tn = in / h;
 }
 
+// A wave's MT x NTL sums of 16 x 16, from row m0 and column n0 of C on: finished, or written as a split's partial sums.
+template <int DT, int EPI, int MT, int NTL>
+__device__ __forceinline__ void finish_tile(const GemmArgs& a, int z, int split, long long m0, int n0, const f32x4 (&acc)[MT][NTL]) {
+    constexpr int DUAL = EPI == EPI_GATED ? 2 : 1, H = NTL / DUAL;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    if (a.splits > 1) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const long long m = m0 + mt * 16 + i;
+            if (m >= a.M) continue;
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+                const int n = n0 + j * 16 + 4 * g;
+                if (n < a.Np) {
+#pragma unroll
+                    for (int d = 0; d < DUAL; ++d)
+                        *(f32x4*)(a.part + (((long long)split * a.nslot + (DUAL == 2 ? d : z)) * a.M + m) * a.Np + n) = acc[mt][j + d * H];
+                }
+            }
+        }
+        return;
+    }
+    epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const long long m = m0 + mt * 16 + i;
+            if (m >= a.M) continue;
+#pragma unroll
+            for (int j = 0; j < H; ++j)
+                epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads>(a, z, m, n0 + j * 16 + 4 * g, acc[mt][j],
+                                                                            acc[mt][DUAL == 2 ? j + H : j]);
+        }
+    });
+}
+
 // BM x BN sums a workgroup of WM x WN waves.  EPI_GATED: the BN columns are BN / 2 of the gate's and the same of up's, and
 // every wave holds both of its columns, so the product needs no exchange.
 template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool AL>
@@ -299,11 +379,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
     auto fetch = [&](char* sx, char* sw, int t) __attribute__((always_inline)) {
         const int seg = t >= a.nk ? 1 : 0;
         const long long k0 = (long long)(t - (seg ? a.nk : 0)) * TX::KE;
-        const int ix = seg | z, iw = EPI == EPI_GATED ? 0 : (seg | z);
-        const char* bx = a.x[ix] + (LX == LK ? m0 * a.ldx[0] : m0 * ES<DT>);
+        const bool second = seg | z;                     // never a variable index: the arguments would be copied to scratch memory
+        const char* bx = (second ? a.x[1] : a.x[0]) + (LX == LK ? m0 * a.ldx[0] : m0 * ES<DT>);
         const long long nw = LW == LK ? n0 * a.ldw[0] : (long long)n0 * ES<DT>;
         lx.fetch(sx, bx, nullptr, a.ldx[0], k0, a.K, mrows, tid);
-        lw.fetch(sw, a.w[iw] + nw, EPI == EPI_GATED ? a.w[1] + nw : nullptr, a.ldw[0], k0, a.K, nrows, tid);
+        lw.fetch(sw, (EPI != EPI_GATED && second ? a.w[1] : a.w[0]) + nw, EPI == EPI_GATED ? a.w[1] + nw : nullptr, a.ldw[0], k0, a.K, nrows, tid);
     };
     auto land = [&](char* sx, char* sw) __attribute__((always_inline)) {
         lx.land(sx, tid);
@@ -316,12 +396,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
         for (int s = 0; s < 2; ++s) {
             u32x4 fx[MT], fw[NTL];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) fx[i] = read_frag<DT, LX, BM, 1, NT>(sx, lane, wm * MT + i, s);
+            for (int i = 0; i < MT; ++i) fx[i] = read_frag<DT, LX, BM, 1, NT>(sx, lane, 0, wm * MT + i, s);
 #pragma unroll
             for (int j = 0; j < NTL; ++j) {
                 constexpr int H = NTL / DUAL;
-                const int t = DUAL == 2 ? (j / H) * (CN / 16) + wn * H + j % H : wn * NTL + j;
-                fw[j] = read_frag<DT, LW, BN, DUAL, NT>(sw, lane, t, s);
+                fw[j] = read_frag<DT, LW, BN, DUAL, NT>(sw, lane, j / H, wn * H + j % H, s);
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -342,26 +421,99 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
         if (t + 2 < t1) land(sx0, sw0);
     }
 
-    const int i = lane & 15, g = lane >> 4;
-    constexpr int H = NTL / DUAL;
+    finish_tile<DT, EPI>(a, z, split, m0 + wm * (BM / WM), n0 + wn * (CN / WN), acc);
+}
+
+// The same product in 256 x 256 tiles by eight waves of 128 x 64, for operands large enough to give every CU a tile.
+//
+// Two waves share a SIMD.  The lower four and the upper four run half a step apart: while the one half's 32 matrix
+// instructions of a k half have the matrix core, the other half reads its next fragments from LDS and sends for the next
+// tile, and a barrier hands over.  Reads are complete before the barrier, so that when a half starts a tile, the buffer of the
+// tile before it is free for the one after it.
+template <int DT, int LX, int LW, int EPI>
+__global__ __launch_bounds__(512, 2) void gemm_big_kernel(GemmArgs a) {
+    constexpr int BM = 256, BN = 256, WM = 2, WN = 4, NT = 512, DUAL = EPI == EPI_GATED ? 2 : 1;
+    typedef Tile<DT, LX, BM, 1, NT> TX;
+    typedef Tile<DT, LW, BN, DUAL, NT> TW;
+    constexpr int MT = BM / WM / 16, NTL = BN / WN / 16, CN = BN / DUAL, H = NTL / DUAL;
+    __shared__ __attribute__((aligned(1024))) char sx0[TX::BYTES], sw0[TW::BYTES], sx1[TX::BYTES], sw1[TW::BYTES];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 2, wn = wave & 3, z = blockIdx.z, split = blockIdx.y;
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+    const long long m0 = (long long)tm * BM;
+    const int n0 = tn * CN;
+    const int mrows = a.M - m0 < BM ? (int)(a.M - m0) : BM, nrows = a.N - n0 < CN ? a.N - n0 : CN;
+    const int t0 = split * a.per_split, t_all = a.nk * a.nseg, t1 = t0 + a.per_split < t_all ? t0 + a.per_split : t_all;
+
+    Loader<DT, LX, BM, 1, NT, true> lx;
+    Loader<DT, LW, BN, DUAL, NT, true> lw;
+    lx.init(tid, a.ldx[0], mrows);
+    lw.init(tid, a.ldw[0], nrows);
+    f32x4 acc[MT][NTL];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const long long m = m0 + wm * (BM / WM) + mt * 16 + i;
-        if (m >= a.M) continue;
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < H; ++j) {
-            const int n = n0 + wn * (CN / WN) + j * 16 + 4 * g;
-            if (a.splits > 1) {
-                if (n < a.Np) {
+        for (int j = 0; j < NTL; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+    auto fetch = [&](char* sx, char* sw, int t) __attribute__((always_inline)) {
+        const int seg = t >= a.nk ? 1 : 0;
+        const long long k0 = (long long)(t - (seg ? a.nk : 0)) * TX::KE;
+        const bool second = seg | z;                     // never a variable index: the arguments would be copied to scratch memory
+        const char* bx = (second ? a.x[1] : a.x[0]) + (LX == LK ? m0 * a.ldx[0] : m0 * ES<DT>);
+        const long long nw = LW == LK ? n0 * a.ldw[0] : (long long)n0 * ES<DT>;
+        lx.fetch(sx, bx, nullptr, a.ldx[0], k0, a.K, mrows, tid);
+        lw.fetch(sw, (EPI != EPI_GATED && second ? a.w[1] : a.w[0]) + nw, EPI == EPI_GATED ? a.w[1] + nw : nullptr, a.ldw[0], k0, a.K, nrows, tid);
+    };
+    u32x4 fx[MT], fw[NTL];
+    auto read = [&](const char* sx, const char* sw, int s) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int d = 0; d < DUAL; ++d)
-                        *(f32x4*)(a.part + (((long long)split * a.nslot + (DUAL == 2 ? d : z)) * a.M + m) * a.Np + n) = acc[mt][j + d * H];
-                }
-            } else {
-                epilogue<DT, EPI>(a, z, m, n, acc[mt][j], acc[mt][DUAL == 2 ? j + H : j]);
-            }
+        for (int j = 0; j < NTL; ++j) {
+            fw[j] = read_frag<DT, LW, BN, DUAL, NT>(sw, lane, j / H, wn * H + j % H, s);
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) fx[i] = read_frag<DT, LX, BM, 1, NT>(sx, lane, 0, wm * MT + i, s);
+    };
+    auto turn = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&]() __attribute__((always_inline)) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = mfma_step<DT>(fw[j], fx[i], acc[i][j]);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    // one tile: s*: where it lies, n*: where the next one goes
+    auto tile = [&](char* sx, char* sw, char* nx, char* nw, int t) __attribute__((always_inline)) {
+        if (t + 1 < t1) fetch(nx, nw, t + 1);
+        read(sx, sw, 0);
+        __builtin_amdgcn_s_waitcnt(0xc07f);              // lgkmcnt(0)
+        turn();
+        multiply();
+        turn();
+        read(sx, sw, 1);
+        __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0), lgkmcnt(0): the next tile is there
+        turn();
+        multiply();
+        turn();
+    };
+
+    fetch(sx0, sw0, t0);
+    __builtin_amdgcn_s_waitcnt(0x0070);
+    turn();
+    if (wave >= 4) turn();                               // half a step behind
+    for (int t = t0; t < t1; t += 2) {
+        tile(sx0, sw0, sx1, sw1, t);
+        if (t + 1 < t1) tile(sx1, sw1, sx0, sw0, t + 1);
     }
+    if (wave < 4) turn();                                // every wave has passed as many barriers
+
+    finish_tile<DT, EPI>(a, z, split, m0 + wm * (BM / WM), n0 + wn * (CN / WN), acc);
 }
 
 // Joins the partial sums of the K splits, in their order, and finishes them.  Eight splits' loads are under way at a time:
@@ -389,6 +541,8 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
                 for (int d = 0; d < DUAL; ++d)
                     if (s + b < a.splits) v[d] += t[b][d];
         }
-        epilogue<DT, EPI>(a, z, m, n, v[0], v[1]);
+        epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
+            epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads>(a, z, m, n, v[0], v[1]);
+        });
     }
 }

@@ -80,7 +80,9 @@ __device__ __forceinline__ void finish(const GemmArgs& a, int split, long long m
 #pragma unroll
         for (int d = 0; d < DUAL; ++d) *(f32x4*)(a.part + (((long long)split * DUAL + d) * a.M + m) * a.Np + n) = v[d];
     } else {
-        epilogue<DT, EPI>(a, 0, m, n, v[0], v[1]);
+        epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
+            epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads>(a, 0, m, n, v[0], v[1]);
+        });
     }
 }
 

@@ -140,6 +140,13 @@ def test_gated_ffn_long_sums(engine, dt):
     ffn_case(engine, 4, 2000, 1600, 40, dt, "lrelu", seed=8)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("size", [(4100, 72, 4104, 72), (4100, 4104, 40, 4104), (40, 4104, 2056, 4104)], ids=lambda s: "x".join(map(str, s)))
+def test_gated_ffn_many_tiles(engine, size, dt):
+    """Results large enough for the largest tiles, ragged at every edge, under short sums."""
+    ffn_case(engine, *size, dt, "silu", seed=13)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_gated_ffn_without_tokens(engine, dt):
     dtype = DT[dt]
