@@ -1,21 +1,19 @@
 // rt_block.hip — the network-block operators of the C ABI: the gated feed-forward block and the norms around it, forward and
-// backward (include/rt_is.h).  Kernels: rt_gemm.hpp (matrix cores), rt_norm.hpp (memory bound).
+// backward (include/rt_is.h): checks, plans and launches.  Kernels: rt_gemm.hpp, rt_skinny.hpp (matrix products), rt_norm.hpp.
 //
 // Every call is a few launches on the context's stream, allocates nothing and keeps nothing: what it needs beyond its
 // arguments is the caller's workspace.  So a call can be captured into a graph, and two graphs do not meet unless their
 // caller gives them the same workspace.
 
-#include "rt_internal.hpp"
+#include "rt_block.hpp"
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
 
-namespace {
+using namespace rt_block;
 
-#include "rt_gemm.hpp"
-#include "rt_skinny.hpp"
-#include "rt_norm.hpp"
+namespace {
 
 int failf(rt_ctx* ctx, int code, const char* fmt, ...) {
     char msg[320];
@@ -104,23 +102,10 @@ int check_ws(rt_ctx* ctx, const char* fn, const void* ws, size_t have, size_t ne
 }
 
 // ---- matrix products ----------------------------------------------------------------------------------------------
-struct Product {                // C [M x N] = X W over K, nseg segments, nbatch products side by side
-    int lx, lw, epi;
-    int64_t M, K;
-    int N, nseg, nbatch;
-    int nrun = nbatch;          // of the products side by side, how many are wanted: the plan, and so the bits, are the same
-};
 
-struct Plan {
-    bool skinny;                // rt_skinny.hpp
-    int li;
-    int bm, bn, splits, per_split, nk, tiles_m, tiles_n, nslot, Np;
-    size_t part_bytes;
-};
 
 // Few rows against weights as they lie in memory: the weights' bytes are all the time there is.  Whether the kernel for
 // them can run depends on alignment too, so the workspace covers both.
-constexpr int SKINNY_ROWS = 32, GEMV_ROWS = 4;
 bool skinny_sizes(const Product& p) { return p.M <= SKINNY_ROWS && p.lx == LK && p.lw == LI && p.N % 4 == 0; }
 
 void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
@@ -148,9 +133,14 @@ void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
 int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Plan& pl) {
     pl.skinny = false;
     const int ke = 128 / elem_size(dtype);
-    // 256 x 256 tiles where they fill the chip
-    const int64_t big = ((p.M + 255) / 256) * ((p.N + (p.epi == EPI_GATED ? 127 : 255)) / (p.epi == EPI_GATED ? 128 : 256)) * p.nbatch;
-    pl.bm = pl.bn = al && dtype != RT_F32 && big >= cus ? 256 : 128;
+    // 256 x 256 tiles, one to a CU, take 1.65 us a step (128 bytes of k) by measurement; of 128 x 128 two share a CU and take
+    // 1.0 us.  (256 x 128: 1.25 us, 1.06 PFLOP/s at best; never the choice.)
+    const int half = p.epi == EPI_GATED ? 2 : 1;
+    auto rounds = [&](int b, int slots) {
+        const int64_t n = (p.M + b - 1) / b * ((p.N + b / half - 1) / (b / half)) * p.nbatch;
+        return (double)((n + slots - 1) / slots);
+    };
+    pl.bm = pl.bn = al && dtype != RT_F32 && rounds(256, cus) * 1.65 < rounds(128, 2 * cus) ? 256 : 128;
     const int cn = p.epi == EPI_GATED ? pl.bn / 2 : pl.bn;
     const int64_t tm = (p.M + pl.bm - 1) / pl.bm, tn = (p.N + cn - 1) / cn, nk = (p.K + ke - 1) / ke;
     if (tm * tn > 0x7fffffff || nk * p.nseg > 0x7fffffff)
@@ -171,77 +161,6 @@ int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Pla
     return RT_OK;
 }
 
-// One row for each kernel that a product can run on.
-typedef void (*GemmFn)(GemmArgs);
-template <int DT, int LX, int LW, int EPI>
-GemmFn gemm_fn(bool al) {
-    return al ? gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, true> : gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, false>;
-}
-
-int launch_join(rt_ctx* ctx, hipStream_t st, GemmFn join, int64_t M, int Np, int nbatch, const GemmArgs& a) {
-    // small joins: one wave a workgroup, so that they spread over the CUs
-    const int64_t quads = M * (Np / 4);
-    const int threads = quads < 65536 ? 64 : 256;
-    const int64_t n = (quads + threads - 1) / threads;
-    hipLaunchKernelGGL(join, dim3((unsigned)(n < 8192 ? n : 8192), 1, nbatch), dim3(threads), 0, st, a);
-    HIPCHK(ctx, hipGetLastError());
-    return RT_OK;
-}
-
-template <int DT>
-int launch_product(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a, bool al) {
-    a.M = p.M; a.N = p.N; a.K = p.K; a.nseg = p.nseg; a.nk = pl.nk;
-    a.tiles_m = pl.tiles_m; a.tiles_n = pl.tiles_n;
-    a.splits = pl.splits; a.per_split = pl.per_split; a.Np = pl.Np; a.nslot = pl.nslot;
-    GemmFn fn, join;
-    if (p.epi == EPI_GATED) {
-        fn = gemm_fn<DT, LK, LI, EPI_GATED>(al);
-        join = gemm_join_kernel<DT, EPI_GATED>;
-    } else if (p.epi == EPI_GATED_BWD) {
-        fn = gemm_fn<DT, LK, LK, EPI_GATED_BWD>(al);
-        join = gemm_join_kernel<DT, EPI_GATED_BWD>;
-    } else {
-        fn = p.lx == LI ? gemm_fn<DT, LI, LI, EPI_STORE>(al)
-                        : p.lw == LI ? gemm_fn<DT, LK, LI, EPI_STORE>(al) : gemm_fn<DT, LK, LK, EPI_STORE>(al);
-        join = gemm_join_kernel<DT, EPI_STORE>;
-    }
-    if constexpr (DT != RT_F32) {
-        if (pl.bm == 256)
-            fn = p.epi == EPI_GATED ? gemm_big_kernel<DT, LK, LI, EPI_GATED>
-                 : p.epi == EPI_GATED_BWD ? gemm_big_kernel<DT, LK, LK, EPI_GATED_BWD>
-                 : p.lx == LI ? gemm_big_kernel<DT, LI, LI, EPI_STORE>
-                 : p.lw == LI ? gemm_big_kernel<DT, LK, LI, EPI_STORE> : gemm_big_kernel<DT, LK, LK, EPI_STORE>;
-    }
-    hipLaunchKernelGGL(fn, dim3(pl.tiles_m * pl.tiles_n, pl.splits, p.nrun), dim3(pl.bm == 256 ? 512 : 256), 0, st, a);
-    HIPCHK(ctx, hipGetLastError());
-    return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, p.nrun, a) : RT_OK;
-}
-
-template <int DT, int EPI, int MR>
-GemmFn gemv_fn(int li) {
-    return li == 16 ? gemv_kernel<DT, EPI, MR, 16> : li == 8 ? gemv_kernel<DT, EPI, MR, 8> : gemv_kernel<DT, EPI, MR, 4>;
-}
-
-template <int DT, int EPI>
-GemmFn skinny_fn(int64_t M, int li) {
-    if (M == 1) return gemv_fn<DT, EPI, 1>(li);
-    if (M == 2) return gemv_fn<DT, EPI, 2>(li);
-    if (M <= GEMV_ROWS) return gemv_fn<DT, EPI, GEMV_ROWS>(li);
-    return M <= 16 ? skinny_kernel<DT, EPI, 1> : skinny_kernel<DT, EPI, 2>;
-}
-
-template <int DT>
-int launch_skinny(rt_ctx* ctx, hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a) {
-    a.M = p.M; a.N = p.N; a.K = p.K;
-    a.splits = pl.splits; a.Np = pl.Np; a.nslot = pl.nslot;
-    const bool gated = p.epi == EPI_GATED;
-    const GemmFn fn = gated ? skinny_fn<DT, EPI_GATED>(p.M, pl.li) : skinny_fn<DT, EPI_STORE>(p.M, pl.li);
-    const GemmFn join = gated ? gemm_join_kernel<DT, EPI_GATED> : gemm_join_kernel<DT, EPI_STORE>;
-    hipLaunchKernelGGL(fn, dim3(pl.tiles_n, pl.splits), dim3(64 * SK_WAVES), 0, st, a);
-    HIPCHK(ctx, hipGetLastError());
-    return pl.splits > 1 ? launch_join(ctx, st, join, p.M, pl.Np, 1, a) : RT_OK;
-}
-
 int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, GemmArgs& a) {
     Plan pl;
     const int es = elem_size(dtype), epc = 16 / es;
@@ -254,17 +173,17 @@ int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, Ge
     if (p.epi == EPI_GATED_BWD) a.quads = a.quads && (uintptr_t)a.e[0] % 16 == 0 && (uintptr_t)a.e[1] % 16 == 0 && a.lde % 16 == 0;
     if (skinny_sizes(p) && a.ldw[0] % (4 * es) == 0 && (uintptr_t)a.w[0] % (4 * es) == 0 && (uintptr_t)a.w[1] % (4 * es) == 0) {
         plan_skinny(v.cu_count, dtype, p, pl);
-        if (dtype == RT_F32) return launch_skinny<RT_F32>(ctx, v.stream, p, pl, a);
-        if (dtype == RT_BF16) return launch_skinny<RT_BF16>(ctx, v.stream, p, pl, a);
-        return launch_skinny<RT_F16>(ctx, v.stream, p, pl, a);
+        HIPCHK(ctx, dtype == RT_F32 ? launch_skinny<RT_F32>(v.stream, p, pl, a)
+                    : dtype == RT_BF16 ? launch_skinny<RT_BF16>(v.stream, p, pl, a) : launch_skinny<RT_F16>(v.stream, p, pl, a));
+        return RT_OK;
     }
     bool al = (p.lx == LK ? p.K : p.M) % epc == 0 && (p.lw == LK ? p.K : p.N) % epc == 0 && a.ldx[0] % 16 == 0 && a.ldw[0] % 16 == 0;
     for (int i = 0; i < 2; ++i) al = al && (uintptr_t)a.x[i] % 16 == 0 && (uintptr_t)a.w[i] % 16 == 0;
     const int rc = plan_product(ctx, v.cu_count, dtype, p, al, pl);
     if (rc) return rc;
-    if (dtype == RT_F32) return launch_product<RT_F32>(ctx, v.stream, p, pl, a, al);
-    if (dtype == RT_BF16) return launch_product<RT_BF16>(ctx, v.stream, p, pl, a, al);
-    return launch_product<RT_F16>(ctx, v.stream, p, pl, a, al);
+    HIPCHK(ctx, dtype == RT_F32 ? launch_product<RT_F32>(v.stream, p, pl, a, al)
+                : dtype == RT_BF16 ? launch_product<RT_BF16>(v.stream, p, pl, a, al) : launch_product<RT_F16>(v.stream, p, pl, a, al));
+    return RT_OK;
 }
 
 // rows x bytes of zeros: a weight gradient of no tokens.
@@ -484,45 +403,9 @@ int norm_make(rt_ctx* ctx, const char* fn, const rt_block_norm* in, int cus, Nor
     return RT_OK;
 }
 
-template <int DT, bool AL, int TPR, int NV>
-void launch_norm(hipStream_t st, const NormArgs& a) {
-    constexpr int B = norm_block(TPR), RPB = B / TPR;
-    hipLaunchKernelGGL((norm_kernel<DT, TPR, NV, AL>), dim3((unsigned)((a.T + RPB - 1) / RPB)), dim3(B), 0, st, a);
-}
-
-template <int DT, bool AL, int TPR, int NV>
-void launch_norm_back(hipStream_t st, const NormArgs& a) {
-    hipLaunchKernelGGL((norm_back_kernel<DT, TPR, NV, AL>), dim3((unsigned)a.units), dim3(norm_block(TPR)), 0, st, a);
-}
-
-template <int DT, bool AL>
-void pick_norm(hipStream_t st, const NormArgs& a, int tpr, bool back) {
-    const int nv = ((a.d + EPC<DT> - 1) / EPC<DT> + tpr - 1) / tpr;
-    if (back) {
-        constexpr int PER = DT == RT_F32 ? 2 : 1;
-        if (tpr == 64) nv <= 1 ? launch_norm_back<DT, AL, 64, 1>(st, a) : launch_norm_back<DT, AL, 64, PER>(st, a);
-        else if (tpr == 256) nv <= 1 ? launch_norm_back<DT, AL, 256, 1>(st, a) : launch_norm_back<DT, AL, 256, PER>(st, a);
-        else if (tpr == 512) nv <= 1 ? launch_norm_back<DT, AL, 512, 1>(st, a) : launch_norm_back<DT, AL, 512, 2>(st, a);
-        else if (nv <= 2) launch_norm_back<DT, AL, 1024, 2>(st, a);
-        else launch_norm_back<DT, AL, 1024, 4>(st, a);
-    } else if (tpr == 64) {
-        if (nv <= 1) launch_norm<DT, AL, 64, 1>(st, a);
-        else if (nv <= 2) launch_norm<DT, AL, 64, 2>(st, a);
-        else launch_norm<DT, AL, 64, 4>(st, a);
-    } else if (tpr == 256) {
-        if (nv <= 1) launch_norm<DT, AL, 256, 1>(st, a);
-        else if (nv <= 2) launch_norm<DT, AL, 256, 2>(st, a);
-        else launch_norm<DT, AL, 256, 4>(st, a);
-    } else {
-        nv <= 2 ? launch_norm<DT, AL, 1024, 2>(st, a) : launch_norm<DT, AL, 1024, 4>(st, a);
-    }
-}
-
 int run_norm(rt_ctx* ctx, hipStream_t st, int dtype, const NormArgs& a, int tpr, bool back, bool al) {
-    if (dtype == RT_F32) al ? pick_norm<RT_F32, true>(st, a, tpr, back) : pick_norm<RT_F32, false>(st, a, tpr, back);
-    else if (dtype == RT_BF16) al ? pick_norm<RT_BF16, true>(st, a, tpr, back) : pick_norm<RT_BF16, false>(st, a, tpr, back);
-    else al ? pick_norm<RT_F16, true>(st, a, tpr, back) : pick_norm<RT_F16, false>(st, a, tpr, back);
-    HIPCHK(ctx, hipGetLastError());
+    HIPCHK(ctx, dtype == RT_F32 ? launch_norm<RT_F32>(st, a, tpr, back, al)
+                : dtype == RT_BF16 ? launch_norm<RT_BF16>(st, a, tpr, back, al) : launch_norm<RT_F16>(st, a, tpr, back, al));
     return RT_OK;
 }
 
@@ -753,11 +636,9 @@ int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_
     const bool gates_left = r.dgate && a.rows_per_gate > m.rows_per_unit;
     const int first = k.want_post || k.want_pre ? 0 : 2, last = gates_left ? 2 + (int)gates : 2;
     if (last > first) {
-        const dim3 grid((a.d + 31) / 32, last - first);
-        if (a.dtype == RT_F32) hipLaunchKernelGGL(norm_join_kernel<RT_F32>, grid, dim3(1024), 0, v.stream, k, first);
-        else if (a.dtype == RT_BF16) hipLaunchKernelGGL(norm_join_kernel<RT_BF16>, grid, dim3(1024), 0, v.stream, k, first);
-        else hipLaunchKernelGGL(norm_join_kernel<RT_F16>, grid, dim3(1024), 0, v.stream, k, first);
-        HIPCHK(ctx, hipGetLastError());
+        HIPCHK(ctx, a.dtype == RT_F32 ? launch_norm_join<RT_F32>(v.stream, k, first, last)
+                    : a.dtype == RT_BF16 ? launch_norm_join<RT_BF16>(v.stream, k, first, last)
+                                         : launch_norm_join<RT_F16>(v.stream, k, first, last));
     }
     return RT_OK;
 }

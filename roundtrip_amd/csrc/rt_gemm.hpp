@@ -9,29 +9,6 @@
 #pragma once
 #include "rt_elem.hpp"
 
-enum { LK = 0, LI = 1 };
-enum { EPI_STORE = 0, EPI_GATED = 1, EPI_GATED_BWD = 2 };
-
-struct GemmArgs {
-    const char* x[2];              // two K segments (nseg = 2), or one operand for each blockIdx.z
-    const char* w[2];              // ... EPI_GATED: gate and up
-    long long ldx[2], ldw[2];      // bytes
-    long long M, K;
-    int N;
-    int nseg;                      // K segments: C = x[0] w[0] + x[1] w[1]
-    int nk;                        // K tiles of a segment
-    int tiles_m, tiles_n;
-    int splits, per_split;         // K tiles are dealt to blockIdx.y, per_split each
-    float* part;                   // splits > 1: [split][slot][M][Np] partial sums, joined by gemm_join_kernel
-    int Np, nslot;
-    char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two float32 or NULL).
-    long long ldo[3];              // (EPI_STORE: ldo[0] for both)  EPI_GATED_BWD: dgate, dup, h
-    const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept, float32
-    long long lde;
-    int act;
-    float alpha;
-    int quads;                     // N and every output's (and e's) place are multiples of four elements
-};
 
 // ---- the gate's activation ----------------------------------------------------------------------------------------
 // s(t) = 1 / (1 + exp(-t)).  16-bit results: hardware exp2 and reciprocal (each <= 1 ulp of float32, far below the
@@ -69,6 +46,36 @@ __device__ __forceinline__ void put4(char* p, f32x4 v, int valid) {
     else store4<DT>(p, v, valid);
 }
 
+// The kept gate and up at four places (columns behind N: nothing).
+template <bool QUADS>
+__device__ __forceinline__ void kept4(const GemmArgs& a, long long m, int n, f32x4& g, f32x4& u) {
+    const int valid = a.N - n;
+    if (valid <= 0) return;
+    const char *pg = a.e[0] + m * a.lde + (long long)n * 4, *pu = a.e[1] + m * a.lde + (long long)n * 4;
+    g = QUADS ? *(const f32x4*)pg : load4<RT_F32>(pg, valid);
+    u = QUADS ? *(const f32x4*)pu : load4<RT_F32>(pu, valid);
+}
+
+// EPI_GATED_BWD: v is dh.
+template <int DT, int ACT, bool QUADS>
+__device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int n, f32x4 v, f32x4 g, f32x4 u) {
+    const int valid = a.N - n;
+    if (valid <= 0) return;
+    const long long c = (long long)n * ES<DT>;
+    f32x4 dg, du, h;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float t, d;
+        act_f<DT, ACT>(a.alpha, g[j], t, d);
+        dg[j] = v[j] * u[j] * d;
+        du[j] = v[j] * t;
+        h[j] = t * u[j];
+    }
+    put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, dg, valid);
+    put4<DT, QUADS>(a.o[1] + m * a.ldo[1] + c, du, valid);
+    put4<DT, QUADS>(a.o[2] + m * a.ldo[2] + c, h, valid);
+}
+
 // What becomes of four neighbouring sums of row m, columns n .. n+3 (v1: the second of EPI_GATED).
 template <int DT, int EPI, int ACT, bool QUADS>
 __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, int n, f32x4 v0, f32x4 v1) {
@@ -91,20 +98,9 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, 
             put4<RT_F32, QUADS>(a.o[2] + m * a.ldo[2] + c4, v1, valid);
         }
     } else {
-        const char *pg = a.e[0] + m * a.lde + c4, *pu = a.e[1] + m * a.lde + c4;
-        const f32x4 g = QUADS ? *(const f32x4*)pg : load4<RT_F32>(pg, valid), u = QUADS ? *(const f32x4*)pu : load4<RT_F32>(pu, valid);
-        f32x4 dg, du, h;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float t, d;
-            act_f<DT, ACT>(a.alpha, g[j], t, d);
-            dg[j] = v0[j] * u[j] * d;
-            du[j] = v0[j] * t;
-            h[j] = t * u[j];
-        }
-        put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, dg, valid);
-        put4<DT, QUADS>(a.o[1] + m * a.ldo[1] + c, du, valid);
-        put4<DT, QUADS>(a.o[2] + m * a.ldo[2] + c, h, valid);
+        f32x4 g, u;
+        kept4<QUADS>(a, m, n, g, u);
+        epilogue_bwd<DT, ACT, QUADS>(a, m, n, v0, g, u);
     }
 }
 
@@ -192,21 +188,54 @@ struct Tile {
     }
 };
 
+// v as a number of 128 bits, shifted down by so many bytes.
+__device__ __forceinline__ u32x4 shift_down(u32x4 v, int bytes) {
+    const int d = bytes >> 2;
+    unsigned w[8] = {v[0], v[1], v[2], v[3], 0, 0, 0, 0}, x[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) x[i] = d == 0 ? w[i] : d == 1 ? w[i + 1] : d == 2 ? w[i + 2] : d == 3 ? w[i + 3] : 0;
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_alignbyte(x[i + 1], x[i], bytes & 3);
+    return r;
+}
+
 template <int DT, int L, int R, int NSUB, int NT, bool AL>
 struct Loader {
     typedef Tile<DT, L, R, NSUB, NT> T;
-    int voff[T::ITER];                // AL: byte offset from the tile's start; OOB where the row or column does not exist
-    u32x4 reg[AL ? 1 : T::ITER];      // !AL: chunks on their way through registers
+    int voff[T::ITER];                // byte offset from the tile's start.  AL: OOB where the row or column does not exist
+    // !AL: chunks go through registers.  A chunk that is not whole is loaded so that it ends where its row does, from earlier
+    // columns on, and shifted into place (zeros follow); rows that do not exist repeat the last.  So loads have no branches.
+    bool ragged, tiny;                // the last chunk of columns is not whole; a row is shorter than a chunk
+    bool on_way, fix;                 // the tile's chunks are in reg; some have to be shifted
+    int had;                          // the k's it has
+    u32x4 reg[AL ? 1 : T::ITER];
 
-    // rows: how many of the tile's rows (LI: columns) exist, counted in a sub-tile
-    __device__ __forceinline__ void init(int tid, long long ld, int rows) {
-        if (!AL) return;
+    // Elements that chunk it lacks at its end, of `rows` columns (LI) or `ke` k's (LK, LI).
+    static __device__ __forceinline__ int lacks(int tid, int it, int rows, int ke) {
+        int sub, idx, c;
+        T::place(tid, it, sub, idx, c);
+        if (L == LI && idx >= ke) return EPC<DT>;
+        const int n = (c + 1) * EPC<DT> - (L == LK ? ke : rows);
+        return n > 0 ? n : 0;
+    }
+
+    // rows: how many of the tile's rows (LI: columns) exist, counted in a sub-tile; all: how many elements a row of the operand has
+    __device__ __forceinline__ void init(int tid, long long ld, int rows, long long all) {
+        ragged = L == LI && rows % (T::SR) != 0;
+        tiny = all < EPC<DT>;
 #pragma unroll
         for (int it = 0; it < T::ITER; ++it) {
             int sub, idx, c;
             T::place(tid, it, sub, idx, c);
-            const int row = L == LK ? idx : c * EPC<DT>;
-            voff[it] = row < rows ? (int)(idx * ld) + c * 16 : OOB;
+            if (AL) {
+                const int row = L == LK ? idx : c * EPC<DT>;
+                voff[it] = row < rows ? (int)(idx * ld) + c * 16 : OOB;
+            } else if (L == LK) {
+                voff[it] = (int)((idx < rows ? idx : rows - 1) * ld) + c * 16;
+            } else {
+                voff[it] = (int)(idx * ld) + c * 16 - lacks(tid, it, rows, T::KE) * ES<DT>;
+            }
         }
     }
 
@@ -238,8 +267,27 @@ struct Loader {
                 }
                 load_to_lds(r, sm + (it * NT + wave * 64) * 16, v);
             }
-        } else {
+        } else if (!tiny) {
+            on_way = true;
+            had = ke;
+            fix = ragged || ke < T::KE;
+            const char *b0 = base + adv, *b1 = (NSUB == 2 ? base2 : base) + adv;
+            if (ke == T::KE) {
 #pragma unroll
+                for (int it = 0; it < T::ITER; ++it) reg[it] = ((const Chunk16*)((NSUB == 2 && it >= T::ITER / 2 ? b1 : b0) + voff[it]))->v;
+            } else {
+                asm volatile("" : "+v"(tid));
+#pragma unroll
+                for (int it = 0; it < T::ITER; ++it) {
+                    int sub, idx, c;
+                    T::place(tid, it, sub, idx, c);
+                    const long long less = L == LK ? lacks(tid, it, rows, ke) * ES<DT> : idx >= ke ? (idx - ke + 1) * ld : 0;
+                    reg[it] = ((const Chunk16*)((NSUB == 2 && it >= T::ITER / 2 ? b1 : b0) + (voff[it] - less)))->v;
+                }
+            }
+        } else {
+            on_way = false;
+#pragma unroll 1
             for (int it = 0; it < T::ITER; ++it) {
                 int sub, idx, c;
                 T::place(tid, it, sub, idx, c);
@@ -247,13 +295,18 @@ struct Loader {
                 const int have = L == LK ? (idx < rows ? ke - c * EPC<DT> : 0) : (idx < ke ? rows - c * EPC<DT> : 0);
                 u32x4 r = {0, 0, 0, 0};
                 if (have > 0) r = load_chunk<DT, false>(b + idx * ld + c * 16, have);
-                reg[it] = r;
+                *(u32x4*)(sm + (it * NT + tid) * 16) = r;
             }
         }
     }
 
-    __device__ __forceinline__ void land(char* sm, int tid) {
-        if (AL) return;
+    __device__ __forceinline__ void land(char* sm, int tid, int rows) {
+        if (AL || !on_way) return;
+        if (fix) {
+            asm volatile("" : "+v"(tid));                // worked out here when it is needed, not held in registers all the time
+#pragma unroll
+            for (int it = 0; it < T::ITER; ++it) reg[it] = shift_down(reg[it], lacks(tid, it, rows, had) * ES<DT>);
+        }
 #pragma unroll
         for (int it = 0; it < T::ITER; ++it) *(u32x4*)(sm + (it * NT + tid) * 16) = reg[it];
     }
@@ -335,14 +388,35 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& a, int z, int split,
         return;
     }
     epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
+        constexpr int ACT = decltype(way)::act;
+        constexpr bool QUADS = decltype(way)::quads;
+        if constexpr (EPI == EPI_GATED_BWD) {            // what it reads is asked for a row of tiles ahead
+            f32x4 gate[2][H], up[2][H];
+            auto ask = [&](int mt) __attribute__((always_inline)) {
+                const long long m = m0 + mt * 16 + i;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const long long m = m0 + mt * 16 + i;
-            if (m >= a.M) continue;
+                for (int j = 0; j < H; ++j)
+                    if (m < a.M) kept4<QUADS>(a, m, n0 + j * 16 + 4 * g, gate[mt & 1][j], up[mt & 1][j]);
+            };
+            ask(0);
 #pragma unroll
-            for (int j = 0; j < H; ++j)
-                epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads>(a, z, m, n0 + j * 16 + 4 * g, acc[mt][j],
-                                                                            acc[mt][DUAL == 2 ? j + H : j]);
+            for (int mt = 0; mt < MT; ++mt) {
+                if (mt + 1 < MT) ask(mt + 1);
+                const long long m = m0 + mt * 16 + i;
+                if (m >= a.M) continue;
+#pragma unroll
+                for (int j = 0; j < H; ++j)
+                    epilogue_bwd<DT, ACT, QUADS>(a, m, n0 + j * 16 + 4 * g, acc[mt][j], gate[mt & 1][j], up[mt & 1][j]);
+            }
+        } else {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const long long m = m0 + mt * 16 + i;
+                if (m >= a.M) continue;
+#pragma unroll
+                for (int j = 0; j < H; ++j)
+                    epilogue<DT, EPI, ACT, QUADS>(a, z, m, n0 + j * 16 + 4 * g, acc[mt][j], acc[mt][DUAL == 2 ? j + H : j]);
+            }
         }
     });
 }
@@ -350,7 +424,7 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& a, int z, int split,
 // BM x BN sums a workgroup of WM x WN waves.  EPI_GATED: the BN columns are BN / 2 of the gate's and the same of up's, and
 // every wave holds both of its columns, so the product needs no exchange.
 template <int DT, int LX, int LW, int EPI, int BM, int BN, int WM, int WN, bool AL>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs a) {
     constexpr int NT = 64 * WM * WN, DUAL = EPI == EPI_GATED ? 2 : 1;
     typedef Tile<DT, LX, BM, 1, NT> TX;
     typedef Tile<DT, LW, BN, DUAL, NT> TW;
@@ -368,8 +442,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
 
     Loader<DT, LX, BM, 1, NT, AL> lx;
     Loader<DT, LW, BN, DUAL, NT, AL> lw;
-    lx.init(tid, a.ldx[0], mrows);
-    lw.init(tid, a.ldw[0], nrows);
+    lx.init(tid, a.ldx[0], mrows, LX == LK ? a.K : a.M);
+    lw.init(tid, a.ldw[0], nrows, LW == LK ? a.K : a.N);
     f32x4 acc[MT][NTL];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -386,14 +460,15 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs a) {
         lw.fetch(sw, (EPI != EPI_GATED && second ? a.w[1] : a.w[0]) + nw, EPI == EPI_GATED ? a.w[1] + nw : nullptr, a.ldw[0], k0, a.K, nrows, tid);
     };
     auto land = [&](char* sx, char* sw) __attribute__((always_inline)) {
-        lx.land(sx, tid);
-        lw.land(sw, tid);
+        lx.land(sx, tid, mrows);
+        lw.land(sw, tid, nrows);
         __builtin_amdgcn_s_waitcnt(0x0f70);          // vmcnt(0): the chunks on their way to LDS have arrived
         __syncthreads();
     };
     auto compute = [&](const char* sx, const char* sw) __attribute__((always_inline)) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
+            if (!AL && s) __builtin_amdgcn_sched_barrier(0);      // the chunks on their way need the registers of a second set
             u32x4 fx[MT], fw[NTL];
 #pragma unroll
             for (int i = 0; i < MT; ++i) fx[i] = read_frag<DT, LX, BM, 1, NT>(sx, lane, 0, wm * MT + i, s);
@@ -439,7 +514,7 @@ __global__ __launch_bounds__(512, 2) void gemm_big_kernel(GemmArgs a) {
     __shared__ __attribute__((aligned(1024))) char sx0[TX::BYTES], sw0[TW::BYTES], sx1[TX::BYTES], sw1[TW::BYTES];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 2, wn = wave & 3, z = blockIdx.z, split = blockIdx.y;
+    const int wm = wave / WN, wn = wave % WN, z = blockIdx.z, split = blockIdx.y;
     int tm, tn;
     tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
     const long long m0 = (long long)tm * BM;
@@ -449,8 +524,8 @@ __global__ __launch_bounds__(512, 2) void gemm_big_kernel(GemmArgs a) {
 
     Loader<DT, LX, BM, 1, NT, true> lx;
     Loader<DT, LW, BN, DUAL, NT, true> lw;
-    lx.init(tid, a.ldx[0], mrows);
-    lw.init(tid, a.ldw[0], nrows);
+    lx.init(tid, a.ldx[0], mrows, LX == LK ? a.K : a.M);
+    lw.init(tid, a.ldw[0], nrows, LW == LK ? a.K : a.N);
     f32x4 acc[MT][NTL];
 #pragma unroll
     for (int i = 0; i < MT; ++i)

@@ -9,26 +9,6 @@
 #pragma once
 #include "rt_elem.hpp"
 
-struct NormArgs {
-    long long T;
-    int d, kind;
-    float eps, rs, bs, w_off;
-    long long rpg;                                   // rows of x that share a row of gate
-    const char *x, *b, *gate, *w_post, *w_pre, *yin; // yin: backward: y, or x where there is no branch
-    char *y, *n;
-    long long ldx, ldb, ldy, ldn, ldg;               // bytes
-    // backward
-    const char *dy, *dn;
-    char *dx, *db, *dgate;
-    long long lddy, lddn, lddx, lddb, lddg;
-    float yin_scale;                                 // y = yin_scale * yin
-    int want_post, want_pre;
-    long long rows_per_unit;                         // consecutive rows of one workgroup
-    int units;
-    int together;                                    // the waves of a workgroup share its rows' gate sums
-    float *p_post, *p_pre, *p_gate;                  // [units][d], [units][d], [units][2][d] partial sums
-    char *dw_post, *dw_pre;
-};
 
 // A wave's sum in all its lanes, the same bits in each: within sixteen lanes by data-parallel moves, then across the rows of
 // sixteen.  (ds_bpermute takes ten times as long a step, and a row waits for three such sums.)

@@ -10,8 +10,6 @@
 #pragma once
 #include "rt_gemm.hpp"
 
-constexpr int SK_WAVES = 8;
-
 // What a step brings of W and X: rows k0 + 8 g + j of the lane's four columns, and the same k's of XR rows of X.
 template <int DT, int DUAL, int XR, int KS>
 struct SkinnyStep {
@@ -89,7 +87,6 @@ __device__ __forceinline__ void finish(const GemmArgs& a, int split, long long m
 // Up to 16 MT rows, 64 columns a workgroup, on the matrix cores.  In a step of 32 k's lane (g = lane / 16, i = lane % 16)
 // holds columns 4 i .. of rows 8 g ..: for one of the four columns the eight rows are an operand of one 16x16x32 instruction
 // as they are (16-bit: after one v_perm for every two values), so nothing passes through LDS.
-constexpr int SK_COLS = 64;
 template <int DT, int EPI, int MT>
 __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(GemmArgs a) {
     constexpr int DUAL = EPI == EPI_GATED ? 2 : 1, NW = SK_WAVES, TILES = MT;

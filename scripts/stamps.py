@@ -1,5 +1,5 @@
 """Diagnostic: per-phase cycle shares of the fused kernel (workgroup 0), from a -DRT_STAMPS build.
-Build here:  hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -mllvm -amdgpu-mfma-vgpr-form -Xclang -target-feature -Xclang -packed-fp32-ops -DRT_STAMPS -o build_diag/librt_is_stamps.so roundtrip_amd/csrc/rt_is.hip roundtrip_amd/csrc/rt_block.hip
+Build here:  hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -mllvm -amdgpu-mfma-vgpr-form -Xclang -target-feature -Xclang -packed-fp32-ops -DRT_STAMPS -o build_diag/librt_is_stamps.so roundtrip_amd/csrc/*.hip
 Run on the GPU box:  RT_IS_LIB=build_diag/librt_is_stamps.so python scripts/stamps.py [dx dy [g_hidden]]
 """
 import ctypes as C, os, sys
