@@ -133,15 +133,27 @@ void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
 int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Plan& pl) {
     pl.skinny = false;
     const int ke = 128 / elem_size(dtype);
-    // 256 x 256 tiles, one to a CU, take 1.65 us a step (128 bytes of k) by measurement; of 128 x 128 two share a CU and take
-    // 1.0 us.  (256 x 128: 1.25 us, 1.06 PFLOP/s at best; never the choice.)
+    // Three tiles: 256 x 256, 128 x 128, 64 x 64 columns of C (the gate's and up's count as one: 128, 64, 64).  Which is quickest
+    // follows from how many fill the CUs how often and what one step (128 bytes of k) costs, by measurement:
+    //   16-bit: one 256 x 256 on a CU 1.65 us, two 128 x 128 side by side 1.0 us, four 64 x 64 1.0 us (bound by LDS);
+    //   float32: by the matrix core alone, 7.4 us for 128 x 128, in proportion to the tile whatever lies side by side.
     const int half = p.epi == EPI_GATED ? 2 : 1;
-    auto rounds = [&](int b, int slots) {
-        const int64_t n = (p.M + b - 1) / b * ((p.N + b / half - 1) / (b / half)) * p.nbatch;
+    auto rounds = [&](int bm, int cn, int slots) {
+        const int64_t n = (p.M + bm - 1) / bm * ((p.N + cn - 1) / cn) * p.nbatch;
         return (double)((n + slots - 1) / slots);
     };
-    pl.bm = pl.bn = al && dtype != RT_F32 && rounds(256, cus) * 1.65 < rounds(128, 2 * cus) ? 256 : 128;
-    const int cn = p.epi == EPI_GATED ? pl.bn / 2 : pl.bn;
+    double t256, t128, t64;
+    if (dtype == RT_F32) {
+        t256 = 1e30;
+        t128 = rounds(128, 128 / half, cus) * 4;
+        t64 = rounds(64, 64, cus) * half * 1.05;
+    } else {
+        t256 = al ? rounds(256, 256 / half, cus) * 1.65 : 1e30;
+        t128 = rounds(128, 128 / half, 2 * cus) * 1.0;
+        t64 = rounds(64, 64, 4 * cus / half) * 1.0;
+    }
+    pl.bm = t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
+    const int cn = pl.bm == 64 ? 64 : pl.bm / half;
     const int64_t tm = (p.M + pl.bm - 1) / pl.bm, tn = (p.N + cn - 1) / cn, nk = (p.K + ke - 1) / ke;
     if (tm * tn > 0x7fffffff || nk * p.nseg > 0x7fffffff)
         return failf(ctx, RT_EUNSUPPORTED, "a product of %lld x %d over %lld is larger than one launch covers", (long long)p.M, p.N,

@@ -61,7 +61,7 @@ struct Product {                // C [M x N] = X W over K, nseg segments, nbatch
 struct Plan {
     bool skinny;                // rt_skinny.hpp
     int li;
-    int bm, bn, splits, per_split, nk, tiles_m, tiles_n, nslot, Np;
+    int bm, splits, per_split, nk, tiles_m, tiles_n, nslot, Np;
     size_t part_bytes;
 };
 

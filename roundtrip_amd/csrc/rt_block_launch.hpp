@@ -11,7 +11,12 @@ namespace {
 // One row for each kernel that a product can run on.
 typedef void (*GemmFn)(GemmArgs);
 template <int DT, int LX, int LW, int EPI>
-GemmFn gemm_fn(bool al) {
+GemmFn gemm_fn(bool al, int bm) {
+    if constexpr (DT != RT_F32) {
+        if (bm == 256) return gemm_big_kernel<DT, LX, LW, EPI>;
+    }
+    constexpr int SMALL_N = EPI == EPI_GATED ? 128 : 64;          // 64 columns of C
+    if (bm == 64) return al ? gemm_kernel<DT, LX, LW, EPI, 64, SMALL_N, 2, 2, true> : gemm_kernel<DT, LX, LW, EPI, 64, SMALL_N, 2, 2, false>;
     return al ? gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, true> : gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, false>;
 }
 
@@ -67,22 +72,15 @@ hipError_t launch_product(hipStream_t st, const Product& p, const Plan& pl, Gemm
     a.splits = pl.splits; a.per_split = pl.per_split; a.Np = pl.Np; a.nslot = pl.nslot;
     GemmFn fn, join;
     if (p.epi == EPI_GATED) {
-        fn = gemm_fn<DT, LK, LI, EPI_GATED>(al);
+        fn = gemm_fn<DT, LK, LI, EPI_GATED>(al, pl.bm);
         join = gemm_join_kernel<DT, EPI_GATED>;
     } else if (p.epi == EPI_GATED_BWD) {
-        fn = gemm_fn<DT, LK, LK, EPI_GATED_BWD>(al);
+        fn = gemm_fn<DT, LK, LK, EPI_GATED_BWD>(al, pl.bm);
         join = gemm_join_kernel<DT, EPI_GATED_BWD>;
     } else {
-        fn = p.lx == LI ? gemm_fn<DT, LI, LI, EPI_STORE>(al)
-                        : p.lw == LI ? gemm_fn<DT, LK, LI, EPI_STORE>(al) : gemm_fn<DT, LK, LK, EPI_STORE>(al);
+        fn = p.lx == LI ? gemm_fn<DT, LI, LI, EPI_STORE>(al, pl.bm)
+                        : p.lw == LI ? gemm_fn<DT, LK, LI, EPI_STORE>(al, pl.bm) : gemm_fn<DT, LK, LK, EPI_STORE>(al, pl.bm);
         join = gemm_join_kernel<DT, EPI_STORE>;
-    }
-    if constexpr (DT != RT_F32) {
-        if (pl.bm == 256)
-            fn = p.epi == EPI_GATED ? gemm_big_kernel<DT, LK, LI, EPI_GATED>
-                 : p.epi == EPI_GATED_BWD ? gemm_big_kernel<DT, LK, LK, EPI_GATED_BWD>
-                 : p.lx == LI ? gemm_big_kernel<DT, LI, LI, EPI_STORE>
-                 : p.lw == LI ? gemm_big_kernel<DT, LK, LI, EPI_STORE> : gemm_big_kernel<DT, LK, LK, EPI_STORE>;
     }
     hipLaunchKernelGGL(fn, dim3(pl.tiles_m * pl.tiles_n, pl.splits, p.nrun), dim3(pl.bm == 256 ? 512 : 256), 0, st, a);
     const hipError_t e = hipGetLastError();
