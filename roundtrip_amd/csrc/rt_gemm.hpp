@@ -342,13 +342,29 @@ template <int DT>
 __device__ __forceinline__ f32x4 mfma_step(u32x4 w, u32x4 x, f32x4 c) {
     if constexpr (DT == RT_BF16)
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, x), c, 0, 0, 0);
-    else if constexpr (DT == RT_F16)
+    else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x), c, 0, 0, 0);
-    else {
-        const f32x4 wf = __builtin_bit_cast(f32x4, w), xf = __builtin_bit_cast(f32x4, x);
+}
+
+// acc[i][j] += W fragment j times X fragment i.  float32 takes four instructions a fragment; the same sums' come as far apart
+// as can be, so that none waits for the one before it.
+template <int DT, int MT, int NTL>
+__device__ __forceinline__ void mfma_tile(const u32x4 (&fw)[NTL], const u32x4 (&fx)[MT], f32x4 (&acc)[MT][NTL]) {
+    if constexpr (DT == RT_F32) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[j], xf[j], c, 0, 0, 0);
-        return c;
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) {
+                    const f32x4 w = __builtin_bit_cast(f32x4, fw[j]), x = __builtin_bit_cast(f32x4, fx[i]);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[q], x[q], acc[i][j], 0, 0, 0);
+                }
+    } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] = mfma_step<DT>(fw[j], fx[i], acc[i][j]);
     }
 }
 
@@ -477,10 +493,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm_kernel(GemmArgs a) {
                 constexpr int H = NTL / DUAL;
                 fw[j] = read_frag<DT, LW, BN, DUAL, NT>(sw, lane, j / H, wn * H + j % H, s);
             }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NTL; ++j) acc[i][j] = mfma_step<DT>(fw[j], fx[i], acc[i][j]);
+            mfma_tile<DT>(fw, fx, acc);
         }
     };
 
@@ -557,10 +570,7 @@ __global__ __launch_bounds__(512, 2) void gemm_big_kernel(GemmArgs a) {
     };
     auto multiply = [&]() __attribute__((always_inline)) {
         __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NTL; ++j) acc[i][j] = mfma_step<DT>(fw[j], fx[i], acc[i][j]);
+        mfma_tile<DT>(fw, fx, acc);
         __builtin_amdgcn_s_setprio(0);
     };
     // one tile: s*: where it lies, n*: where the next one goes
