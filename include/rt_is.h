@@ -320,6 +320,8 @@ typedef struct rt_gated_ffn {
     const void *w_gate, *w_up;   /* d_in x d_ff, both with stride ld_in */
     const void *w_down;          /* d_ff x d_out */
     void *out;                   /* T x d_out */
+    const void *x_lo;            /* 16-bit types: T x d_in with x's stride, or NULL: x + x_lo is what is multiplied by w_gate and
+                                    w_up (rt_block_norm's n and n_lo); dw_gate and dw_up are of x alone */
     float *pre_gate, *pre_up;    /* T x d_ff float32 in every dtype: x w_gate and x w_up, kept for the backward pass (rounded
                                     to 16 bits they would double the error of every gradient); both NULL if there is none */
 } rt_gated_ffn;
@@ -362,6 +364,8 @@ typedef struct rt_block_norm {
     const void *gate;            /* ceil(T / rows_per_gate) x d or NULL */
     const void *w_post, *w_pre;  /* d or NULL */
     void *y, *n;                 /* T x d; one of them may be NULL; each may be x's or branch's own memory, row for row */
+    void *n_lo;                  /* 16-bit types: T x d with n's stride, or NULL: what n's rounding left off, so that n + n_lo has
+                                    twice the digits.  A gate's sign hangs on them: leaky ReLU's slope jumps at 0. */
 } rt_block_norm;
 
 /* Gradients of sum(dy * y) + sum(dn * n).  dy or dn may be NULL (zeros); a NULL output is not computed. */

@@ -52,7 +52,7 @@ class RtGatedFfn(C.Structure):
     as the addresses in it hold."""
     _fields_ = ([(k, C.c_int32) for k in ("dtype", "act", "d_in", "d_ff", "d_out")] + [("alpha", C.c_float)]
                 + [(k, C.c_int64) for k in ("T", "ldx", "ld_in", "ld_down", "ld_out", "ld_pre")]
-                + [(k, C.c_void_p) for k in ("x", "w_gate", "w_up", "w_down", "out", "pre_gate", "pre_up")])
+                + [(k, C.c_void_p) for k in ("x", "w_gate", "w_up", "w_down", "out", "x_lo", "pre_gate", "pre_up")])
 
 
 class RtGatedFfnGrads(C.Structure):
@@ -65,7 +65,7 @@ class RtBlockNorm(C.Structure):
     _fields_ = ([(k, C.c_int32) for k in ("dtype", "kind", "d")]
                 + [(k, C.c_float) for k in ("eps", "res_scale", "branch_scale", "w_offset")]
                 + [(k, C.c_int64) for k in ("T", "rows_per_gate", "ldx", "ld_branch", "ldy", "ldn", "ld_gate")]
-                + [(k, C.c_void_p) for k in ("x", "branch", "gate", "w_post", "w_pre", "y", "n")])
+                + [(k, C.c_void_p) for k in ("x", "branch", "gate", "w_post", "w_pre", "y", "n", "n_lo")])
 
 
 class RtBlockNormGrads(C.Structure):
@@ -397,11 +397,11 @@ class Engine(object):
 
     @staticmethod
     def gated_ffn_args(T, d_in, d_ff, d_out, dtype, act, x=None, w_gate=None, w_up=None, w_down=None, out=None,
-                       pre_gate=None, pre_up=None, alpha=0.2, ldx=0, ld_in=0, ld_down=0, ld_out=0, ld_pre=0):
+                       pre_gate=None, pre_up=None, x_lo=None, alpha=0.2, ldx=0, ld_in=0, ld_down=0, ld_out=0, ld_pre=0):
         """out = (act(x w_gate) * (x w_up)) w_down; pre_gate / pre_up keep what the backward pass needs."""
         return RtGatedFfn(dtype=dtype, act=act, d_in=d_in, d_ff=d_ff, d_out=d_out, alpha=alpha, T=T, ldx=ldx, ld_in=ld_in,
                           ld_down=ld_down, ld_out=ld_out, ld_pre=ld_pre, x=x, w_gate=w_gate, w_up=w_up, w_down=w_down,
-                          out=out, pre_gate=pre_gate, pre_up=pre_up)
+                          out=out, x_lo=x_lo, pre_gate=pre_gate, pre_up=pre_up)
 
     @staticmethod
     def gated_ffn_grads(dout=None, dx=None, dw_gate=None, dw_up=None, dw_down=None, ld_dout=0, ld_dx=0, ld_dw_in=0,
@@ -422,13 +422,13 @@ class Engine(object):
         self._chk(self._lib.rt_gated_ffn_backward_dev(self._h, C.byref(args), C.byref(grads), ws_ptr, ws_bytes))
 
     @staticmethod
-    def block_norm_args(T, d, dtype, kind, x=None, branch=None, y=None, n=None, w_post=None, w_pre=None, gate=None,
+    def block_norm_args(T, d, dtype, kind, x=None, branch=None, y=None, n=None, n_lo=None, w_post=None, w_pre=None, gate=None,
                         rows_per_gate=1, res_scale=1.0, branch_scale=1.0, eps=1e-5, w_offset=0.0, ldx=0, ld_branch=0, ldy=0,
                         ldn=0, ld_gate=0):
         """y = res_scale x + branch_scale gate * N(branch; w_post), n = N(y; w_pre)."""
         return RtBlockNorm(dtype=dtype, kind=kind, d=d, eps=eps, res_scale=res_scale, branch_scale=branch_scale,
                            w_offset=w_offset, T=T, rows_per_gate=rows_per_gate, ldx=ldx, ld_branch=ld_branch, ldy=ldy, ldn=ldn,
-                           ld_gate=ld_gate, x=x, branch=branch, gate=gate, w_post=w_post, w_pre=w_pre, y=y, n=n)
+                           ld_gate=ld_gate, x=x, branch=branch, gate=gate, w_post=w_post, w_pre=w_pre, y=y, n=n, n_lo=n_lo)
 
     @staticmethod
     def block_norm_grads(dy=None, dn=None, dx=None, dbranch=None, dgate=None, dw_post=None, dw_pre=None, ld_dy=0, ld_dn=0,

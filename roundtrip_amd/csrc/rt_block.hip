@@ -243,6 +243,7 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
     rt_gated_ffn& a = f.a;
     if (a.dtype != RT_F32 && a.dtype != RT_BF16 && a.dtype != RT_F16) return failf(ctx, RT_EINVAL, "%s: unknown dtype %d", fn, a.dtype);
     if (a.act < RT_ACT_SILU || a.act > RT_ACT_SIGMOID) return failf(ctx, RT_EINVAL, "%s: unknown activation %d", fn, a.act);
+    if (a.x_lo && a.dtype == RT_F32) return failf(ctx, RT_EINVAL, "%s: x_lo is for 16-bit types", fn);
     if (!isfinite(a.alpha)) return failf(ctx, RT_EINVAL, "%s: alpha is not finite", fn);
     if (a.T < 0 || a.T > MAX_ROWS) return failf(ctx, RT_EINVAL, "%s: T = %lld", fn, (long long)a.T);
     if (a.d_in < 1 || a.d_ff < 1 || a.d_out < 1 || a.d_in > MAX_DIM || a.d_ff > MAX_DIM || a.d_out > MAX_DIM)
@@ -255,7 +256,7 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
     if (!a.ld_pre) a.ld_pre = a.d_ff;
     f.ldh = up(a.d_ff, 16 / f.es);
     f.h_bytes = (size_t)up(a.T * f.ldh * f.es, 256);
-    f.gated = {LK, LI, EPI_GATED, a.T, a.d_in, a.d_ff, 1, 1};
+    f.gated = {LK, LI, EPI_GATED, a.T, a.d_in, a.d_ff, a.x_lo ? 2 : 1, 1};      // x_lo: another run of k's, of the same weights
     f.down = {LK, LI, EPI_STORE, a.T, a.d_ff, a.d_out, 1, 1};
     f.dh = {LK, LK, EPI_GATED_BWD, a.T, a.d_out, a.d_ff, 1, 1};
     f.dx = {LK, LK, EPI_STORE, a.T, a.d_ff, a.d_in, 2, 1};
@@ -263,10 +264,12 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
     f.dw_down = {LI, LI, EPI_STORE, a.d_ff, a.T, a.d_out, 1, 1};
     f.ws_fwd = f.ws_bwd = 0;
     if (a.T == 0) return RT_OK;
-    // whichever kernels the call's alignment lets it use
+    // whichever kernels the call's alignment lets it use, with and without x_lo
     size_t fwd = 0, bwd = 0;
     int rc;
-    for (const Product* p : {&f.gated, &f.down})
+    Product other = f.gated;
+    other.nseg = 3 - other.nseg;
+    for (const Product* p : {&f.gated, &other, &f.down})
         if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, fwd))) return rc;
     for (const Product* p : {&f.dh, &f.dx, &f.dw_in, &f.dw_down})
         if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, bwd))) return rc;
@@ -299,7 +302,7 @@ int ffn_forward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, char* ws) {
     g.part = (float*)(ws + f.h_bytes);
     g.act = a.act;
     g.alpha = a.alpha;
-    set_x(g, a.x, a.x, a.ldx * es);
+    set_x(g, a.x, a.x_lo ? a.x_lo : a.x, a.ldx * es);
     set_w(g, a.w_gate, a.w_up, a.ld_in * es);
     set_o(g, 0, h, f.ldh * es);
     set_o(g, 1, a.pre_gate, a.ld_pre * 4);
@@ -437,7 +440,7 @@ void norm_args(const Norm& m, NormArgs& k) {
     k.eps = a.eps; k.rs = a.res_scale; k.bs = a.branch_scale; k.w_off = a.w_offset; k.rpg = a.rows_per_gate;
     k.x = (const char*)a.x; k.b = (const char*)a.branch; k.gate = (const char*)a.gate;
     k.w_post = (const char*)a.w_post; k.w_pre = (const char*)a.w_pre;
-    k.y = (char*)a.y; k.n = (char*)a.n;
+    k.y = (char*)a.y; k.n = (char*)a.n; k.n_lo = (char*)a.n_lo;
     k.ldx = a.ldx * es; k.ldb = a.ld_branch * es; k.ldy = a.ldy * es; k.ldn = a.ldn * es; k.ldg = a.ld_gate * es;
 }
 
@@ -476,16 +479,16 @@ int rt_gated_ffn_dev(rt_ctx* ctx, const rt_gated_ffn* args, void* ws, size_t ws_
     if (rc) return rc;
     const rt_gated_ffn& a = f.a;
     const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx, f.es}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in, f.es}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in, f.es},
-                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}};
+                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}, {"x_lo", a.x_lo, a.T, a.d_in, a.ldx, f.es}};
     const Mat out[] = {{"out", a.out, a.T, a.d_out, a.ld_out, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, 4},
                        {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, 4}, {"the workspace", ws, 1, (int64_t)f.ws_fwd, (int64_t)f.ws_fwd, 1}};
-    for (const Mat& m : in)
-        if ((rc = check_mat(ctx, fn, m, true))) return rc;
+    for (int i = 0; i < 5; ++i)
+        if ((rc = check_mat(ctx, fn, in[i], i < 4))) return rc;
     for (int i = 0; i < 3; ++i)
         if ((rc = check_mat(ctx, fn, out[i], i == 0))) return rc;
     if (!a.pre_gate != !a.pre_up) return failf(ctx, RT_EINVAL, "%s: give both of pre_gate and pre_up, or neither", fn);
     if (a.T == 0) return RT_OK;
-    if ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_fwd)) || (rc = check_disjoint(ctx, fn, in, 4, out, 4))) return rc;
+    if ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_fwd)) || (rc = check_disjoint(ctx, fn, in, 5, out, 4))) return rc;
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);
     return ffn_forward(ctx, v, f, (char*)ws);
@@ -553,20 +556,23 @@ int rt_block_norm_dev(rt_ctx* ctx, const rt_block_norm* args) {
     const int64_t gates = (a.T + a.rows_per_gate - 1) / a.rows_per_gate;
     const Mat in[] = {{"x", a.x, a.T, a.d, a.ldx, m.es}, {"branch", a.branch, a.T, a.d, a.ld_branch, m.es}, {"gate", a.gate, gates, a.d, a.ld_gate, m.es},
                       {"w_post", a.w_post, 1, a.d, a.d, m.es}, {"w_pre", a.w_pre, 1, a.d, a.d, m.es}};
-    const Mat out[] = {{"y", a.y, a.T, a.d, a.ldy, m.es}, {"n", a.n, a.T, a.d, a.ldn, m.es}};
+    const Mat out[] = {{"y", a.y, a.T, a.d, a.ldy, m.es}, {"n", a.n, a.T, a.d, a.ldn, m.es}, {"n_lo", a.n_lo, a.T, a.d, a.ldn, m.es}};
     for (int i = 0; i < 5; ++i)
         if ((rc = check_mat(ctx, fn, in[i], i == 0))) return rc;
     for (const Mat& o : out)
         if ((rc = check_mat(ctx, fn, o, false))) return rc;
     if (a.gate && !a.branch) return failf(ctx, RT_EINVAL, "%s: a gate without a branch", fn);
+    if (a.n_lo && (a.dtype == RT_F32 || !a.n)) return failf(ctx, RT_EINVAL, "%s: n_lo is for 16-bit types, beside n", fn);
     if (a.T == 0) return RT_OK;
     if (!a.y && !a.n) return failf(ctx, RT_EINVAL, "%s: y and n are both NULL", fn);
     // rows are read before they are written: an output may take the place of x or of branch, whole
     for (const Mat& o : out)
         for (int i = 0; i < 5; ++i)
-            if (overlap(o, in[i]) && !(i < 2 && same_place(o, in[i])))
+            if (overlap(o, in[i]) && !(i < 2 && &o != &out[2] && same_place(o, in[i])))
                 return failf(ctx, RT_EINVAL, "%s: %s and %s overlap", fn, o.name, in[i].name);
     if (overlap(out[0], out[1])) return failf(ctx, RT_EINVAL, "%s: y and n overlap", fn);
+    for (int i = 0; i < 2; ++i)
+        if (overlap(out[2], out[i])) return failf(ctx, RT_EINVAL, "%s: n_lo and %s overlap", fn, out[i].name);
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);
     NormArgs k;

@@ -35,7 +35,7 @@ struct NormArgs {
     float eps, rs, bs, w_off;
     long long rpg;                                   // rows of x that share a row of gate
     const char *x, *b, *gate, *w_post, *w_pre, *yin; // yin: backward: y, or x where there is no branch
-    char *y, *n;
+    char *y, *n, *n_lo;
     long long ldx, ldb, ldy, ldn, ldg;               // bytes
     // backward
     const char *dy, *dn;
@@ -54,7 +54,7 @@ struct NormArgs {
 struct Product {                // C [M x N] = X W over K, nseg segments, nbatch products side by side
     int lx, lw, epi;
     int64_t M, K;
-    int N, nseg, nbatch;
+    int N = 0, nseg = 1, nbatch = 1;
     int nrun = nbatch;          // of the products side by side, how many are wanted: the plan, and so the bits, are the same
 };
 

@@ -87,17 +87,17 @@ hipError_t launch_product(hipStream_t st, const Product& p, const Plan& pl, Gemm
     return e == hipSuccess && pl.splits > 1 ? launch_join(st, join, p.M, pl.Np, p.nrun, a) : e;
 }
 
-template <int DT, int EPI, int MR>
+template <int DT, int EPI, int MR, bool LO>
 GemmFn gemv_fn(int li) {
-    return li == 16 ? gemv_kernel<DT, EPI, MR, 16> : li == 8 ? gemv_kernel<DT, EPI, MR, 8> : gemv_kernel<DT, EPI, MR, 4>;
+    return li == 16 ? gemv_kernel<DT, EPI, MR, 16, LO> : li == 8 ? gemv_kernel<DT, EPI, MR, 8, LO> : gemv_kernel<DT, EPI, MR, 4, LO>;
 }
 
-template <int DT, int EPI>
+template <int DT, int EPI, bool LO>
 GemmFn skinny_fn(int64_t M, int li) {
-    if (M == 1) return gemv_fn<DT, EPI, 1>(li);
-    if (M == 2) return gemv_fn<DT, EPI, 2>(li);
-    if (M <= GEMV_ROWS) return gemv_fn<DT, EPI, GEMV_ROWS>(li);
-    return M <= 16 ? skinny_kernel<DT, EPI, 1> : skinny_kernel<DT, EPI, 2>;
+    if (M == 1) return gemv_fn<DT, EPI, 1, LO>(li);
+    if (M == 2) return gemv_fn<DT, EPI, 2, LO>(li);
+    if (M <= GEMV_ROWS) return gemv_fn<DT, EPI, GEMV_ROWS, LO>(li);
+    return M <= 16 ? skinny_kernel<DT, EPI, 1, LO> : skinny_kernel<DT, EPI, 2, LO>;
 }
 
 template <int DT>
@@ -105,7 +105,10 @@ hipError_t launch_skinny(hipStream_t st, const Product& p, const Plan& pl, GemmA
     a.M = p.M; a.N = p.N; a.K = p.K;
     a.splits = pl.splits; a.Np = pl.Np; a.nslot = pl.nslot;
     const bool gated = p.epi == EPI_GATED;
-    const GemmFn fn = gated ? skinny_fn<DT, EPI_GATED>(p.M, pl.li) : skinny_fn<DT, EPI_STORE>(p.M, pl.li);
+    GemmFn fn = gated ? skinny_fn<DT, EPI_GATED, false>(p.M, pl.li) : skinny_fn<DT, EPI_STORE, false>(p.M, pl.li);
+    if constexpr (DT != RT_F32) {
+        if (gated && p.nseg == 2) fn = skinny_fn<DT, EPI_GATED, true>(p.M, pl.li);
+    }
     const GemmFn join = gated ? gemm_join_kernel<DT, EPI_GATED> : gemm_join_kernel<DT, EPI_STORE>;
     hipLaunchKernelGGL(fn, dim3(pl.tiles_n, pl.splits), dim3(64 * SK_WAVES), 0, st, a);
     const hipError_t e = hipGetLastError();

@@ -199,6 +199,10 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
         v.scale(f);
         if (a.w_pre) v.times(R(mpre), a.w_off);
         v.store(a.n + row * a.ldn, a.d, t);
+        if (a.n_lo) {                            // what the rounding left off
+            FOR_ROW(k, e) v.v[k][e] -= (float)(typename Elem<DT>::T)v.v[k][e];
+            v.store(a.n_lo + row * a.ldn, a.d, t);
+        }
     }
 }
 

@@ -11,12 +11,13 @@
 #include "rt_gemm.hpp"
 
 // What a step brings of W and X: rows k0 + 8 g + j of the lane's four columns, and the same k's of XR rows of X.
-template <int DT, int DUAL, int XR, int KS>
+// LO: of X and of what its rounding left off.
+template <int DT, int DUAL, int XR, int KS, bool LO>
 struct SkinnyStep {
     typedef typename Elem<DT>::T T;
     struct __attribute__((aligned(4 * ES<DT>))) Four { T t[4]; };
     Four w[DUAL][8];
-    u32x4 x[XR][8 / EPC<DT>];
+    u32x4 x[XR][8 / EPC<DT>], lo[LO ? XR : 1];
 
     // at: where the lane's columns and its first row lie from a row that is the same for the whole wave.  Row t of x is
     // m0 + t * mstep of X; rows behind M repeat the last (their sums are dropped).
@@ -47,6 +48,15 @@ struct SkinnyStep {
                 } else {
                     x[t][h] = u32x4{0, 0, 0, 0};
                     if (k + h * EPC<DT> < K) x[t][h] = load_chunk<DT, false>(p + 16 * h, K - k - h * EPC<DT>);
+                }
+            }
+            if (LO) {
+                const char* q = a.x[1] + m * a.ldx[0] + (long long)k * ES<DT>;
+                if (whole) {
+                    lo[t] = ((const Chunk16*)q)->v;
+                } else {
+                    lo[t] = u32x4{0, 0, 0, 0};
+                    if (k < K) lo[t] = load_chunk<DT, false>(q, K - k);
                 }
             }
         }
@@ -87,10 +97,10 @@ __device__ __forceinline__ void finish(const GemmArgs& a, int split, long long m
 // Up to 16 MT rows, 64 columns a workgroup, on the matrix cores.  In a step of 32 k's lane (g = lane / 16, i = lane % 16)
 // holds columns 4 i .. of rows 8 g ..: for one of the four columns the eight rows are an operand of one 16x16x32 instruction
 // as they are (16-bit: after one v_perm for every two values), so nothing passes through LDS.
-template <int DT, int EPI, int MT>
+template <int DT, int EPI, int MT, bool LO>
 __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(GemmArgs a) {
     constexpr int DUAL = EPI == EPI_GATED ? 2 : 1, NW = SK_WAVES, TILES = MT;
-    typedef SkinnyStep<DT, DUAL, TILES, 32> Step;
+    typedef SkinnyStep<DT, DUAL, TILES, 32, LO> Step;
     __shared__ float sm[NW][DUAL][SK_COLS / 4][16][4];         // [wave][..][quad of columns][row][column]: one row tile
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * SK_COLS, split = blockIdx.y, K = (int)a.K, steps = (K + 31) >> 5;
@@ -127,7 +137,10 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(GemmArgs a) {
                         w[j] = __builtin_amdgcn_perm(c < 2 ? hi.x : hi.y, c < 2 ? lo.x : lo.y, c & 1 ? 0x07060302u : 0x05040100u);
                     }
 #pragma unroll
-                    for (int t = 0; t < TILES; ++t) acc[t][d][c] = mfma_step<DT>(w, s.x[t][0], acc[t][d][c]);
+                    for (int t = 0; t < TILES; ++t) {
+                        acc[t][d][c] = mfma_step<DT>(w, s.x[t][0], acc[t][d][c]);
+                        if constexpr (LO) acc[t][d][c] = mfma_step<DT>(w, s.lo[t], acc[t][d][c]);
+                    }
                 }
             }
     };
@@ -166,10 +179,10 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(GemmArgs a) {
 // Up to MR <= 4 rows on the vector unit, 4 LI columns a workgroup.  With one row the chip is kept busy by many narrow slabs (a
 // CU alone draws some 60 GB/s of weights), and a matrix instruction would be used for a sixteenth of its rows; float32's takes
 // 32 cycles for four k's whatever they are.  Lane (g, i), i < LI, holds columns 4 i .. of rows 8 g .. of a step of 512 / LI k's.
-template <int DT, int EPI, int MR, int LI>
+template <int DT, int EPI, int MR, int LI, bool LO>
 __global__ __launch_bounds__(64 * SK_WAVES) void gemv_kernel(GemmArgs a) {
     constexpr int DUAL = EPI == EPI_GATED ? 2 : 1, G = 64 / LI, KS = 8 * G;
-    typedef SkinnyStep<DT, DUAL, MR, KS> Step;
+    typedef SkinnyStep<DT, DUAL, MR, KS, LO> Step;
     __shared__ float sm[SK_WAVES][DUAL][MR][LI][4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane % LI, g = lane / LI;
     // neighbouring slabs share cache lines where they are narrow: give them to one XCD
@@ -196,6 +209,11 @@ __global__ __launch_bounds__(64 * SK_WAVES) void gemv_kernel(GemmArgs a) {
                 chunk_to_f32<DT>(s.x[m][h], f);
 #pragma unroll
                 for (int e = 0; e < EPC<DT>; ++e) x[m][h * EPC<DT> + e] = f[e];
+                if constexpr (LO) {
+                    chunk_to_f32<DT>(s.lo[m], f);
+#pragma unroll
+                    for (int e = 0; e < EPC<DT>; ++e) x[m][e] += f[e];
+                }
             }
 #pragma unroll
         for (int d = 0; d < DUAL; ++d)

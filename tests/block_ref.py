@@ -113,7 +113,10 @@ def norm(x, b, gate, rpg, w_post, w_pre, kind, eps, rs, bs, off, dtype):
         ev = ev + eb * f.abs() + 6 * F * ((bh * f).abs() + v.abs())
     vh, _, evh, _ = hat(kind, v, ev, eps)
     w = one if w_pre is None else w_pre + off
-    return {"y": rounded(v, ev, dtype), "n": rounded(vh * w, evh * w.abs() + 4 * F * (vh * w).abs(), dtype)}
+    n, en = vh * w, evh * w.abs() + 4 * F * (vh * w).abs()
+    u, sub = half_step(dtype)
+    # n's rounding leaves off at most u of it, that part's own rounding u of that
+    return {"y": rounded(v, ev, dtype), "n": rounded(n, en, dtype), "n_and_lo": (n, en + 2 * u * u * (n.abs() + en) + 2 * sub)}
 
 
 def through_hat(kind, z, ez, vh, evh, r, er):

@@ -65,6 +65,8 @@ WS = C.c_void_p(BASE + (1 << 30))
     (dict(pre_up=BASE + (1 << 28)), EINVAL, "both of pre_gate"), (dict(out=BASE), EINVAL, "out and x overlap"),
     (dict(out=BASE + 318), EINVAL, "out and x overlap"), (dict(out=BASE + (1 << 24) + 64), EINVAL, "out and w_gate overlap"),
     (dict(pre_gate=BASE + (1 << 28), pre_up=BASE + (1 << 28) + 4), EINVAL, "overlap"), (dict(pre_gate=BASE + (1 << 28) + 2, pre_up=BASE + (1 << 27)), EINVAL, "pre_gate is not aligned"), (dict(out=WS.value), EINVAL, "workspace and out overlap"),
+    (dict(dtype=0, x_lo=BASE + (1 << 26) + (1 << 25)), EINVAL, "x_lo is for 16-bit"), (dict(x_lo=BASE + (1 << 26) + (1 << 25) + 1), EINVAL, "x_lo is not aligned"),
+    (dict(x_lo=BASE + 4 * (1 << 24) + 8), EINVAL, "out and x_lo overlap"),
     (dict(T=1 << 38, d_ff=1 << 20, d_in=1 << 20), EUNSUPPORTED, "one launch")])
 def test_gated_ffn_refusals(lib, kw, code, words):
     a = ffn(**kw)
@@ -121,7 +123,9 @@ def norm(**kw):
     (dict(ld_gate=10), EINVAL, "row stride of gate"), (dict(ldx=1 << 21), EUNSUPPORTED, "row stride of x"), (dict(x=BASE + 2), EINVAL, "aligned"),
     (dict(y=BASE + 4), EINVAL, "y and x overlap"), (dict(y=BASE, ldy=65), EINVAL, "y and x overlap"), (dict(n=BASE + (1 << 24) + 256), EINVAL, "n and branch overlap"),
     (dict(n=BASE + (1 << 25)), EINVAL, "y and n overlap"), (dict(y=BASE + (1 << 26)), EINVAL, "y and gate overlap"),
-    (dict(n=BASE + 5 * (1 << 24)), EINVAL, "n and w_post overlap")])
+    (dict(n=BASE + 5 * (1 << 24)), EINVAL, "n and w_post overlap"), (dict(n_lo=BASE + (1 << 27)), EINVAL, "n_lo is for 16-bit"),
+    (dict(dtype=1, n=None, n_lo=BASE + (1 << 27)), EINVAL, "n_lo is for 16-bit"), (dict(dtype=1, n_lo=BASE), EINVAL, "n_lo and x overlap"),
+    (dict(dtype=1, n_lo=BASE + 3 * (1 << 24) + 2), EINVAL, "n_lo and n overlap")])
 def test_block_norm_refusals(lib, kw, code, words):
     a = norm(**kw)
     refused(lib, lib.rt_block_norm_dev(lib.ctx, C.byref(a)), code, words)

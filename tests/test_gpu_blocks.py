@@ -47,10 +47,11 @@ def workspace(n):
     return torch.full((max(n, 16),), 0xA5, dtype=torch.uint8, device="cuda")
 
 
-def ffn_case(engine, T, di, f, do, dt, act, lds=(0, 0, 0, 0, 0), shift=0, alpha=0.2, seed=0):
+def ffn_case(engine, T, di, f, do, dt, act, lds=(0, 0, 0, 0, 0), shift=0, alpha=0.2, seed=0, lo=False):
     """Runs forward and backward and checks every output."""
     dtype, gen = DT[dt], torch.Generator().manual_seed(seed)
     x, x64 = normal(gen, (T, di), dtype)
+    xl, xl64 = normal(gen, (T, di), dtype, 2.0 ** -9) if lo else (None, 0.0)
     wg, wg64 = normal(gen, (di, f), dtype, 1.5 * di ** -0.5)
     wu, wu64 = normal(gen, (di, f), dtype, di ** -0.5)
     wd, wd64 = normal(gen, (f, do), dtype, f ** -0.5)
@@ -59,17 +60,18 @@ def ffn_case(engine, T, di, f, do, dt, act, lds=(0, 0, 0, 0, 0), shift=0, alpha=
     A = lambda r, w, l=None, v=None: Array(r, w, dtype, l, shift, v)  # noqa: E731
     ax, ag, au, ad = A(T, di, ld[0], x), A(di, f, ld[1], wg), A(di, f, ld[1], wu), A(f, do, ld[2], wd)
     ao, ado = A(T, do, ld[3]), A(T, do, ld[3], dout)
+    al = A(T, di, ld[0], xl) if lo else None
     pg, pu = Array(T, f, torch.float32, ld[4], shift), Array(T, f, torch.float32, ld[4], shift)
     for keep in (False, True):
         a = engine.gated_ffn_args(T, di, f, do, CODE[dt], ACT[act], x=ax.ptr, w_gate=ag.ptr, w_up=au.ptr, w_down=ad.ptr,
-                                  out=ao.ptr, pre_gate=pg.ptr if keep else None, pre_up=pu.ptr if keep else None, alpha=alpha,
+                                  out=ao.ptr, pre_gate=pg.ptr if keep else None, pre_up=pu.ptr if keep else None, alpha=alpha, x_lo=al.ptr if lo else None,
                                   ldx=ld[0], ld_in=ld[1], ld_down=ld[2], ld_out=ld[3], ld_pre=ld[4])
         n = engine.gated_ffn_workspace(a)
         ws = workspace(n)
         torch.cuda.synchronize()
         engine.gated_ffn_dev(a, ws.data_ptr(), n)
         engine.sync()
-        want = ref.ffn(x64, wg64, wu64, wd64, act, alpha, dtype)
+        want = ref.ffn(x64 + xl64, wg64, wu64, wd64, act, alpha, dtype)
         ref.check(ao.view, want["out"], "out")
         if keep:
             ref.check(pg.view, want["pre_gate"], "pre_gate")
@@ -131,6 +133,14 @@ def test_gated_ffn_activations(engine, act, dt):
 def test_gated_ffn_strides_and_alignment(engine, dt, lds, shift):
     ffn_case(engine, 70, 64, 128, 96, dt, "silu", lds, shift, seed=5)
     ffn_case(engine, 5, 64, 128, 96, dt, "gelu", lds, shift, seed=6)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("size", [(1, 64, 128, 64), (2, 70, 256, 8), (3, 2000, 96, 5), (16, 128, 256, 128), (31, 72, 104, 40), (100, 130, 96, 66), (300, 512, 512, 64),
+                                  (7, 33, 57, 31), (4100, 72, 4104, 16)], ids=lambda s: "x".join(map(str, s)))
+def test_gated_ffn_with_the_rest_of_x(engine, size, dt):
+    """x_lo: the gate's and up's sums are those of x + x_lo."""
+    ffn_case(engine, *size, dt, "lrelu", seed=14, lo=True)
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
@@ -263,7 +273,8 @@ def norm_case(engine, T, d, dt, kind, rpg, branch=True, post=True, pre=True, rs=
     ax, ab, ag = A(T, ld[0], x), opt(T, ld[1], b), opt(G, ld[4], gate)
     aw, av = opt(1, d, wpo), opt(1, d, wpr)
     y, n = A(T, ld[2]) if want_y else None, A(T, ld[3]) if want_n else None
-    a = engine.block_norm_args(T, d, CODE[dt], KIND[kind], x=ax.ptr, branch=ptr(ab), y=ptr(y), n=ptr(n), w_post=ptr(aw), w_pre=ptr(av),
+    nl = A(T, ld[3]) if want_n and dt != "f32" else None
+    a = engine.block_norm_args(T, d, CODE[dt], KIND[kind], x=ax.ptr, branch=ptr(ab), y=ptr(y), n=ptr(n), n_lo=ptr(nl), w_post=ptr(aw), w_pre=ptr(av),
                                gate=ptr(ag), rows_per_gate=rpg, res_scale=rs, branch_scale=bs, eps=eps, w_offset=off, ldx=ld[0],
                                ld_branch=ld[1], ldy=ld[2], ldn=ld[3], ld_gate=ld[4])
     torch.cuda.synchronize()
@@ -275,6 +286,18 @@ def norm_case(engine, T, d, dt, kind, rpg, branch=True, post=True, pre=True, rs=
         if arr is not None:
             ref.check(arr.view, want[k], k)
             assert arr.untouched_outside(), k
+    if nl is not None:
+        ref.check(n.view.double() + nl.view.double(), want["n_and_lo"], "n + n_lo")
+        assert nl.untouched_outside()
+        plain = A(T, ld[3])                       # without it n is the same
+        a.n, a.n_lo = plain.ptr, None
+        if y is not None:
+            a.y = None
+        torch.cuda.synchronize()
+        engine.block_norm_dev(a)
+        engine.sync()
+        assert torch.equal(plain.view, n.view)
+        a.y = ptr(y)
     # backward, at a y of its own
     dy, dy64 = normal(gen, (T, d), dtype) if want_y else (None, None)
     dn, dn64 = normal(gen, (T, d), dtype) if want_n else (None, None)
@@ -424,8 +447,12 @@ class Block(object):
             t["d" + k] = torch.empty_like(t[k])
         p = {k: v.data_ptr() for k, v in t.items()}
         code = CODE[dt]
-        self.before = engine.block_norm_args(T, d, code, KIND["rms"], x=p["x"], n=p["h"], w_pre=p["w_in"])
-        self.ffn = engine.gated_ffn_args(T, d, f, d, code, ACT["silu"], x=p["h"], w_gate=p["w_gate"], w_up=p["w_up"], w_down=p["w_down"],
+        p["lo"] = None
+        if dt != "f32":
+            t["lo"] = new(T, d)
+            p["lo"] = t["lo"].data_ptr()
+        self.before = engine.block_norm_args(T, d, code, KIND["rms"], x=p["x"], n=p["h"], n_lo=p["lo"], w_pre=p["w_in"])
+        self.ffn = engine.gated_ffn_args(T, d, f, d, code, ACT["silu"], x=p["h"], x_lo=p["lo"], w_gate=p["w_gate"], w_up=p["w_up"], w_down=p["w_down"],
                                          out=p["b"], pre_gate=p["pg"], pre_up=p["pu"])
         self.after = engine.block_norm_args(T, d, code, KIND["rms"], x=p["x"], branch=p["b"], y=p["y"], n=p["n"], w_post=p["w_post"],
                                             w_pre=p["w_pre"], gate=p["gate"], rows_per_gate=3)
