@@ -152,7 +152,9 @@ def prepare(case, seed):
         x = s["x"] if case["op"] == "ffn" else new(T, d)
         b = new(T, d)
         s["pre"] = [torch.empty((T, f), device="cuda") if train else None for _ in range(2)]       # float32 in every type
-        s["ffn"] = eng.gated_ffn_args(T, d, f, d, code, act, x=p(x), w_gate=p(s["w_gate"]), w_up=p(s["w_up"]),
+        # the norm before hands over what its rounding left off too: the sign of a gate hangs on it
+        lo = s["lo"] = new(T, d) if case["op"] == "block" and case["dtype"] != "f32" else None
+        s["ffn"] = eng.gated_ffn_args(T, d, f, d, code, act, x=p(x), x_lo=p(lo), w_gate=p(s["w_gate"]), w_up=p(s["w_up"]),
                                       w_down=p(s["w_down"]), out=p(b), pre_gate=p(s["pre"][0]), pre_up=p(s["pre"][1]),
                                       alpha=ALPHA)
         ws = eng.gated_ffn_workspace(s["ffn"])
@@ -190,7 +192,7 @@ def prepare(case, seed):
             ws = max(ws, eng.block_norm_workspace(s["norm"]))
         if case["op"] == "block":
             # the norm before: of the block's input, with no branch; its gradient joins the residual's
-            s["norm_in"] = eng.block_norm_args(T, d, code, kind, x=p(s["x"]), n=p(x), w_pre=p(s["w_in"]), eps=EPS)
+            s["norm_in"] = eng.block_norm_args(T, d, code, kind, x=p(s["x"]), n=p(x), n_lo=p(lo), w_pre=p(s["w_in"]), eps=EPS)
             if train:
                 out["dw_in"] = new(d)
                 s["norm_in_grads"] = eng.block_norm_grads(dy=p(dx), dn=p(s["keep"][1]), dx=p(dx),
