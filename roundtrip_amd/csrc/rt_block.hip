@@ -133,42 +133,44 @@ void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
 int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Plan& pl) {
     pl.skinny = false;
     const int ke = 128 / elem_size(dtype);
-    // Three tiles: 256 x 256, 128 x 128, 64 x 64 columns of C (the gate's and up's count as one: 128, 64, 64).  Which is quickest
-    // follows from how many fill the CUs how often and what one step (128 bytes of k) costs, by measurement:
-    //   16-bit: one 256 x 256 on a CU 1.65 us, two 128 x 128 side by side 1.0 us, four 64 x 64 1.0 us (bound by LDS);
-    //   float32: by the matrix core alone, 7.4 us for 128 x 128, in proportion to the tile whatever lies side by side.
+    // Three tiles: 256 x 256, 128 x 128, 64 x 64 columns of C (the gate's and up's count as one: 128, 64, 64), and K split over s
+    // workgroups.  With L workgroups side by side on a CU (at most `fit`, what its LDS holds) a step (128 bytes of k) takes the
+    // larger of `least`, what one workgroup waits for memory and barriers, and L * `each`, what the matrix core (16-bit tiles
+    // below 256: LDS) needs; splits are joined by another launch, which reads what they wrote.  By measurement, in us:
+    //   16-bit: 256 x 256 1.65 / 1.65;  128 x 128 0.7 / 0.5;  64 x 64 0.7 / 0.25        float32: 128 x 128 2.2 / 1.9;  64 x 64 0.8 / 0.5
+    struct Size { int bm, cn, fit; double least, each; };
     const int half = p.epi == EPI_GATED ? 2 : 1;
-    auto rounds = [&](int bm, int cn, int slots) {
-        const int64_t n = (p.M + bm - 1) / bm * ((p.N + cn - 1) / cn) * p.nbatch;
-        return (double)((n + slots - 1) / slots);
-    };
-    double t256, t128, t64;
-    if (dtype == RT_F32) {
-        t256 = 1e30;
-        t128 = rounds(128, 128 / half, cus) * 4;
-        t64 = rounds(64, 64, cus) * half * 1.05;
-    } else {
-        t256 = al ? rounds(256, 256 / half, cus) * 1.65 : 1e30;
-        t128 = rounds(128, 128 / half, 2 * cus) * 1.0;
-        t64 = rounds(64, 64, 4 * cus / half) * 1.0;
+    const bool f32 = dtype == RT_F32;
+    const Size sizes[3] = {{64, 64, half == 2 ? 3 : 5, f32 ? 0.8 : 0.7, (f32 ? 0.5 : 0.25) * half},
+                           {128, 128 / half, 2, f32 ? 2.2 : 0.7, f32 ? 1.9 : 0.5}, {256, 256 / half, 1, 1.65, 1.65}};
+    pl.nslot = p.epi == EPI_GATED ? 2 : p.nbatch;
+    pl.Np = (int)up(p.N, 4);
+    const int64_t nk = (p.K + ke - 1) / ke, steps = nk * p.nseg;
+    double best = 1e300;
+    int64_t tm = 0, tn = 0;
+    for (int i = 0; i < (al && !f32 ? 3 : 2); ++i) {
+        const Size& z = sizes[i];
+        const int64_t m = (p.M + z.bm - 1) / z.bm, n = (p.N + z.cn - 1) / z.cn, tiles = m * n * p.nbatch;
+        for (int64_t k = 1; k <= 32 && (k == 1 || (k * 2 <= steps && tiles * k <= 2 * cus)); k *= 2) {
+            const int64_t per = (steps + k - 1) / k, load = (tiles * k + cus - 1) / cus;
+            const double join = k > 1 ? 5.0 + (double)k * pl.nslot * p.M * pl.Np * 8 / 4.5e6 : 0.0;
+            auto together = [&](int64_t n) { return n * z.each > z.least ? n * z.each : n ? z.least : 0.0; };
+            const double t = per * (load / z.fit * together(z.fit) + together(load % z.fit)) + join;
+            if (t >= best) continue;
+            best = t;
+            pl.bm = z.bm;
+            pl.per_split = (int)per;
+            pl.splits = (int)((steps + per - 1) / per);
+            tm = m;
+            tn = n;
+        }
     }
-    pl.bm = t64 <= t128 && t64 <= t256 ? 64 : t128 <= t256 ? 128 : 256;
-    const int cn = pl.bm == 64 ? 64 : pl.bm / half;
-    const int64_t tm = (p.M + pl.bm - 1) / pl.bm, tn = (p.N + cn - 1) / cn, nk = (p.K + ke - 1) / ke;
-    if (tm * tn > 0x7fffffff || nk * p.nseg > 0x7fffffff)
+    if (tm * tn > 0x7fffffff || steps > 0x7fffffff)
         return failf(ctx, RT_EUNSUPPORTED, "a product of %lld x %d over %lld is larger than one launch covers", (long long)p.M, p.N,
                      (long long)p.K);
     pl.tiles_m = (int)tm;
     pl.tiles_n = (int)tn;
     pl.nk = (int)nk;
-    pl.nslot = p.epi == EPI_GATED ? 2 : p.nbatch;
-    pl.Np = (int)up(p.N, 4);
-    const int64_t tiles = tm * tn * p.nbatch, steps = nk * p.nseg;
-    int64_t s = tiles >= cus ? 1 : cus / tiles;
-    if (s > steps / 4) s = steps / 4;
-    if (s < 1) s = 1;
-    pl.per_split = (int)((steps + s - 1) / s);
-    pl.splits = (int)((steps + pl.per_split - 1) / pl.per_split);
     pl.part_bytes = pl.splits > 1 ? (size_t)pl.splits * pl.nslot * p.M * pl.Np * sizeof(float) : 0;
     return RT_OK;
 }
