@@ -144,7 +144,7 @@ int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Pla
     const Size sizes[3] = {{64, 64, half == 2 ? 3 : 5, f32 ? 0.8 : 0.7, (f32 ? 0.5 : 0.25) * half},
                            {128, 128 / half, 2, f32 ? 2.2 : 0.7, f32 ? 1.9 : 0.5}, {256, 256 / half, 1, 1.65, 1.65}};
     pl.nslot = p.epi == EPI_GATED ? 2 : p.nbatch;
-    pl.Np = (int)up(p.N, 4);
+    pl.Np = (int)up(p.No > p.N ? p.No : p.N, 4);
     const int64_t nk = (p.K + ke - 1) / ke, steps = nk * p.nseg;
     double best = 1e300;
     int64_t tm = 0, tn = 0;
@@ -191,7 +191,7 @@ int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, Ge
                     : dtype == RT_BF16 ? launch_skinny<RT_BF16>(v.stream, p, pl, a) : launch_skinny<RT_F16>(v.stream, p, pl, a));
         return RT_OK;
     }
-    bool al = (p.lx == LK ? p.K : p.M) % epc == 0 && (p.lw == LK ? p.K : p.N) % epc == 0 && a.ldx[0] % 16 == 0 && a.ldw[0] % 16 == 0;
+    bool al = (p.xpad || (p.lx == LK ? p.K : p.M) % epc == 0) && (p.wpad || (p.lw == LK ? p.K : p.N) % epc == 0) && a.ldx[0] % 16 == 0 && a.ldw[0] % 16 == 0;
     for (int i = 0; i < 2; ++i) al = al && (uintptr_t)a.x[i] % 16 == 0 && (uintptr_t)a.w[i] % 16 == 0;
     const int rc = plan_product(ctx, v.cu_count, dtype, p, al, pl);
     if (rc) return rc;
@@ -219,10 +219,14 @@ struct Ffn {
     int es;
     int64_t ldh;                   // elements; h, dgate and dup lie in the workspace
     size_t h_bytes;
+    bool pad;                      // many rows: operands of odd widths are copied, padded
+    size_t pad_x, pad_in, pad_down, pad_dout;      // bytes of a copy, 0: none is needed
     Product gated, down;           // forward
     Product dh, dx, dw_in, dw_down;
-    size_t ws_fwd, ws_bwd;
+    size_t ws_fwd, ws_bwd, part_fwd, part_bwd;
 };
+
+constexpr int PAD_ROWS = 1024;
 
 // Raises `most` to the bytes of partial sums this product can need.
 int most_part_bytes(rt_ctx* ctx, int cus, int dtype, const Product& p, size_t& most) {
@@ -258,12 +262,30 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
     if (!a.ld_pre) a.ld_pre = a.d_ff;
     f.ldh = up(a.d_ff, 16 / f.es);
     f.h_bytes = (size_t)up(a.T * f.ldh * f.es, 256);
+    // Odd widths make every product read its operands unaligned, at half the speed of the kernels for whole chunks; one pass over
+    // them before costs as much as a few hundred rows gain.
+    f.pad = a.T >= PAD_ROWS;
+    const int epc = 16 / f.es;
+    auto copy = [&](int64_t rows, int64_t width) { return f.pad && width % epc ? (size_t)up(rows * up(width, epc) * f.es, 256) : (size_t)0; };
+    f.pad_x = copy(a.T, a.d_in);
+    f.pad_in = copy(a.d_in, a.d_ff);
+    f.pad_down = copy(a.d_ff, a.d_out);
+    f.pad_dout = copy(a.T, a.d_out);
     f.gated = {LK, LI, EPI_GATED, a.T, a.d_in, a.d_ff, a.x_lo ? 2 : 1, 1};      // x_lo: another run of k's, of the same weights
     f.down = {LK, LI, EPI_STORE, a.T, a.d_ff, a.d_out, 1, 1};
     f.dh = {LK, LK, EPI_GATED_BWD, a.T, a.d_out, a.d_ff, 1, 1};
     f.dx = {LK, LK, EPI_STORE, a.T, a.d_ff, a.d_in, 2, 1};
     f.dw_in = {LI, LI, EPI_STORE, a.d_in, a.T, a.d_ff, 1, 2};
     f.dw_down = {LI, LI, EPI_STORE, a.d_ff, a.T, a.d_out, 1, 1};
+    if (f.pad) {
+        // h, dgate and dup are written with zeros behind their rows, and count as padded where they are read
+        f.gated.No = f.dh.No = (int)f.ldh;
+        f.down.xpad = f.dx.xpad = f.dw_down.xpad = f.dw_in.wpad = true;
+        f.gated.xpad = f.dw_in.xpad = f.pad_x;
+        f.gated.wpad = f.dx.wpad = f.pad_in;
+        f.down.wpad = f.dh.wpad = f.pad_down;
+        f.dh.xpad = f.dw_down.wpad = f.pad_dout;
+    }
     f.ws_fwd = f.ws_bwd = 0;
     if (a.T == 0) return RT_OK;
     // whichever kernels the call's alignment lets it use, with and without x_lo
@@ -275,8 +297,11 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
         if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, fwd))) return rc;
     for (const Product* p : {&f.dh, &f.dx, &f.dw_in, &f.dw_down})
         if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, bwd))) return rc;
-    f.ws_fwd = f.h_bytes + fwd;
-    f.ws_bwd = 3 * f.h_bytes + bwd;
+    const size_t copies = 2 * f.pad_x + 2 * f.pad_in + f.pad_down;      // (x_lo too)
+    f.ws_fwd = f.h_bytes + up(fwd, 256) + copies;
+    f.ws_bwd = 3 * f.h_bytes + up(bwd, 256) + copies + f.pad_dout;
+    f.part_fwd = fwd;
+    f.part_bwd = bwd;
     return RT_OK;
 }
 
@@ -295,24 +320,60 @@ void set_o(GemmArgs& g, int i, void* p, int64_t ld) {
     g.ldo[i] = ld;
 }
 
+// Operands as the products read them: the caller's, or padded copies of them at `at` in the workspace.
+struct Operands {
+    const void *x, *x_lo, *w_gate, *w_up, *w_down, *dout;
+    int64_t ldx, ld_in, ld_down, ld_dout;      // bytes
+};
+
+int ffn_operands(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const void* dout, int64_t ld_dout, char* at, Operands& o) {
+    const rt_gated_ffn& a = f.a;
+    const int64_t es = f.es, epc = 16 / es;
+    o = {a.x, a.x_lo, a.w_gate, a.w_up, a.w_down, dout, a.ldx * es, a.ld_in * es, a.ld_down * es, ld_dout * es};
+    PadArgs p;
+    p.n = 0;
+    auto copy = [&](const void*& src, int64_t ld, int64_t rows, int64_t width, size_t bytes) {
+        if (!bytes || !src) return;
+        p.m[p.n++] = {(const char*)src, at, ld, up(width, epc) * es, rows, (int)width};
+        src = at;
+        at += bytes;
+    };
+    copy(o.x, o.ldx, a.T, a.d_in, f.pad_x);
+    if (!dout) copy(o.x_lo, o.ldx, a.T, a.d_in, f.pad_x);
+    copy(o.w_gate, o.ld_in, a.d_in, a.d_ff, f.pad_in);
+    copy(o.w_up, o.ld_in, a.d_in, a.d_ff, f.pad_in);
+    copy(o.w_down, o.ld_down, a.d_ff, a.d_out, f.pad_down);
+    copy(o.dout, o.ld_dout, a.T, a.d_out, f.pad_dout);
+    if (f.pad_x) o.ldx = up(a.d_in, epc) * es;
+    if (f.pad_in) o.ld_in = up(a.d_ff, epc) * es;
+    if (f.pad_down) o.ld_down = up(a.d_out, epc) * es;
+    if (f.pad_dout) o.ld_dout = up(a.d_out, epc) * es;
+    if (p.n)
+        HIPCHK(ctx, a.dtype == RT_F32 ? launch_pad<RT_F32>(v.stream, p) : a.dtype == RT_BF16 ? launch_pad<RT_BF16>(v.stream, p)
+                                                                                              : launch_pad<RT_F16>(v.stream, p));
+    return RT_OK;
+}
+
 int ffn_forward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, char* ws) {
     const rt_gated_ffn& a = f.a;
     const int64_t es = f.es;
     char* h = ws;
+    Operands o;
+    int rc = ffn_operands(ctx, v, f, nullptr, 0, ws + f.h_bytes + up(f.part_fwd, 256), o);
+    if (rc) return rc;
     GemmArgs g;
     memset(&g, 0, sizeof g);
     g.part = (float*)(ws + f.h_bytes);
     g.act = a.act;
     g.alpha = a.alpha;
-    set_x(g, a.x, a.x_lo ? a.x_lo : a.x, a.ldx * es);
-    set_w(g, a.w_gate, a.w_up, a.ld_in * es);
+    set_x(g, o.x, a.x_lo ? o.x_lo : o.x, o.ldx);
+    set_w(g, o.w_gate, o.w_up, o.ld_in);
     set_o(g, 0, h, f.ldh * es);
     set_o(g, 1, a.pre_gate, a.ld_pre * 4);
     set_o(g, 2, a.pre_up, a.ld_pre * 4);
-    int rc = run_product(ctx, v, a.dtype, f.gated, g);
-    if (rc) return rc;
+    if ((rc = run_product(ctx, v, a.dtype, f.gated, g))) return rc;
     set_x(g, h, h, f.ldh * es);
-    set_w(g, a.w_down, a.w_down, a.ld_down * es);
+    set_w(g, o.w_down, o.w_down, o.ld_down);
     set_o(g, 0, a.out, a.ld_out * es);
     return run_product(ctx, v, a.dtype, f.down, g);
 }
@@ -326,10 +387,12 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
     g.part = (float*)(ws + 3 * f.h_bytes);
     g.act = a.act;
     g.alpha = a.alpha;
-    int rc;
+    Operands o;
+    int rc = ffn_operands(ctx, v, f, r.dout, r.ld_dout, ws + 3 * f.h_bytes + up(f.part_bwd, 256), o);
+    if (rc) return rc;
     // dh = dout Wd^T, and from it what the gate's and up's sums get, and h again
-    set_x(g, r.dout, r.dout, r.ld_dout * es);
-    set_w(g, a.w_down, a.w_down, a.ld_down * es);
+    set_x(g, o.dout, o.dout, o.ld_dout);
+    set_w(g, o.w_down, o.w_down, o.ld_down);
     set_o(g, 0, dg, ldh);
     set_o(g, 1, du, ldh);
     set_o(g, 2, h, ldh);
@@ -339,13 +402,13 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
     if ((rc = run_product(ctx, v, a.dtype, f.dh, g))) return rc;
     if (r.dx) {                      // dx = dgate Wg^T + dup Wu^T: one sum over both
         set_x(g, dg, du, ldh);
-        set_w(g, a.w_gate, a.w_up, a.ld_in * es);
+        set_w(g, o.w_gate, o.w_up, o.ld_in);
         set_o(g, 0, r.dx, r.ld_dx * es);
         if ((rc = run_product(ctx, v, a.dtype, f.dx, g))) return rc;
     }
     if (r.dw_gate || r.dw_up) {      // x^T dgate and x^T dup side by side
         Product p = f.dw_in;
-        set_x(g, a.x, a.x, a.ldx * es);
+        set_x(g, o.x, o.x, o.ldx);
         set_w(g, r.dw_gate ? dg : du, r.dw_up ? du : dg, ldh);
         set_o(g, 0, r.dw_gate ? r.dw_gate : r.dw_up, r.ld_dw_in * es);
         set_o(g, 1, r.dw_up, r.ld_dw_in * es);
@@ -354,7 +417,7 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
     }
     if (r.dw_down) {
         set_x(g, h, h, ldh);
-        set_w(g, r.dout, r.dout, r.ld_dout * es);
+        set_w(g, o.dout, o.dout, o.ld_dout);
         set_o(g, 0, r.dw_down, r.ld_dw_down * es);
         if ((rc = run_product(ctx, v, a.dtype, f.dw_down, g))) return rc;
     }

@@ -20,6 +20,7 @@ struct GemmArgs {
     int splits, per_split;         // K tiles are dealt to blockIdx.y, per_split each
     float* part;                   // splits > 1: [split][slot][M][Np] partial sums, joined by gemm_join_kernel
     int Np, nslot;
+    int No;                        // columns written: N, or more of the workspace's own rows, zeros that the next product may read
     char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two float32 or NULL).
     long long ldo[3];              // (EPI_STORE: ldo[0] for both)  EPI_GATED_BWD: dgate, dup, h
     const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept, float32
@@ -55,6 +56,8 @@ struct Product {                // C [M x N] = X W over K, nseg segments, nbatch
     int lx, lw, epi;
     int64_t M, K;
     int N = 0, nseg = 1, nbatch = 1;
+    int No = 0;                 // columns to write, if more than N
+    bool xpad = false, wpad = false;   // the operand's rows are padded with zeros to whole 16-byte chunks
     int nrun = nbatch;          // of the products side by side, how many are wanted: the plan, and so the bits, are the same
 };
 
@@ -68,9 +71,21 @@ struct Plan {
 constexpr int SKINNY_ROWS = 32, GEMV_ROWS = 4;    // rt_skinny.hpp: most rows; most of them on the vector unit
 constexpr int SK_WAVES = 8, SK_COLS = 64;
 
+// Copies of matrices whose rows are no whole number of 16-byte chunks, with zeros behind each row.
+struct PadArgs {
+    int n;
+    struct One {
+        const char* src;
+        char* dst;
+        long long ld, ldd, rows;   // bytes
+        int width;                 // elements
+    } m[5];
+};
+
 // Launches on the element type DT.  Each returns the launches' first error.
 template <int DT> RT_HIDDEN hipError_t launch_product(hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a, bool al);
 template <int DT> RT_HIDDEN hipError_t launch_skinny(hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a);
+template <int DT> RT_HIDDEN hipError_t launch_pad(hipStream_t st, const PadArgs& a);
 template <int DT> RT_HIDDEN hipError_t launch_norm(hipStream_t st, const NormArgs& a, int tpr, bool back, bool al);
 template <int DT> RT_HIDDEN hipError_t launch_norm_join(hipStream_t st, const NormArgs& a, int first, int last);
 

@@ -20,6 +20,19 @@ GemmFn gemm_fn(bool al, int bm) {
     return al ? gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, true> : gemm_kernel<DT, LX, LW, EPI, 128, 128, 2, 2, false>;
 }
 
+// One matrix a blockIdx.y, one 16-byte chunk of the copy a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void pad_kernel(PadArgs a) {
+    const PadArgs::One& m = blockIdx.y == 0 ? a.m[0] : blockIdx.y == 1 ? a.m[1] : blockIdx.y == 2 ? a.m[2] : blockIdx.y == 3 ? a.m[3] : a.m[4];
+    const int chunks = (int)(m.ldd / 16);
+    const long long total = m.rows * chunks;
+    for (long long p = (long long)blockIdx.x * 256 + threadIdx.x; p < total; p += (long long)gridDim.x * 256) {
+        const long long r = p / chunks;
+        const int c = (int)(p - r * chunks);
+        *(u32x4*)(m.dst + r * m.ldd + c * 16) = load_chunk<DT, false>(m.src + r * m.ld + c * 16, m.width - c * EPC<DT>);
+    }
+}
+
 hipError_t launch_join(hipStream_t st, GemmFn join, int64_t M, int Np, int nbatch, const GemmArgs& a) {
     // small joins: one wave a workgroup, so that they spread over the CUs
     const int64_t quads = M * (Np / 4);
@@ -70,6 +83,7 @@ hipError_t launch_product(hipStream_t st, const Product& p, const Plan& pl, Gemm
     a.M = p.M; a.N = p.N; a.K = p.K; a.nseg = p.nseg; a.nk = pl.nk;
     a.tiles_m = pl.tiles_m; a.tiles_n = pl.tiles_n;
     a.splits = pl.splits; a.per_split = pl.per_split; a.Np = pl.Np; a.nslot = pl.nslot;
+    a.No = p.No > p.N ? p.No : p.N;
     GemmFn fn, join;
     if (p.epi == EPI_GATED) {
         fn = gemm_fn<DT, LK, LI, EPI_GATED>(al, pl.bm);
@@ -102,7 +116,7 @@ GemmFn skinny_fn(int64_t M, int li) {
 
 template <int DT>
 hipError_t launch_skinny(hipStream_t st, const Product& p, const Plan& pl, GemmArgs& a) {
-    a.M = p.M; a.N = p.N; a.K = p.K;
+    a.M = p.M; a.N = a.No = p.N; a.K = p.K;
     a.splits = pl.splits; a.Np = pl.Np; a.nslot = pl.nslot;
     const bool gated = p.epi == EPI_GATED;
     GemmFn fn = gated ? skinny_fn<DT, EPI_GATED, false>(p.M, pl.li) : skinny_fn<DT, EPI_STORE, false>(p.M, pl.li);
@@ -113,6 +127,12 @@ hipError_t launch_skinny(hipStream_t st, const Product& p, const Plan& pl, GemmA
     hipLaunchKernelGGL(fn, dim3(pl.tiles_n, pl.splits), dim3(64 * SK_WAVES), 0, st, a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess && pl.splits > 1 ? launch_join(st, join, p.M, pl.Np, 1, a) : e;
+}
+
+template <int DT>
+hipError_t launch_pad(hipStream_t st, const PadArgs& a) {
+    hipLaunchKernelGGL(pad_kernel<DT>, dim3(2048, a.n), dim3(256), 0, st, a);
+    return hipGetLastError();
 }
 
 template <int DT>
@@ -129,6 +149,7 @@ hipError_t launch_norm_join(hipStream_t st, const NormArgs& a, int first, int la
 
 template hipError_t launch_product<RT_BLOCK_DT>(hipStream_t, const Product&, const Plan&, GemmArgs&, bool);
 template hipError_t launch_skinny<RT_BLOCK_DT>(hipStream_t, const Product&, const Plan&, GemmArgs&);
+template hipError_t launch_pad<RT_BLOCK_DT>(hipStream_t, const PadArgs&);
 template hipError_t launch_norm<RT_BLOCK_DT>(hipStream_t, const NormArgs&, int, bool, bool);
 template hipError_t launch_norm_join<RT_BLOCK_DT>(hipStream_t, const NormArgs&, int, int);
 

@@ -50,6 +50,7 @@ __device__ __forceinline__ void put4(char* p, f32x4 v, int valid) {
 template <bool QUADS>
 __device__ __forceinline__ void kept4(const GemmArgs& a, long long m, int n, f32x4& g, f32x4& u) {
     const int valid = a.N - n;
+    g = u = f32x4{0, 0, 0, 0};
     if (valid <= 0) return;
     const char *pg = a.e[0] + m * a.lde + (long long)n * 4, *pu = a.e[1] + m * a.lde + (long long)n * 4;
     g = QUADS ? *(const f32x4*)pg : load4<RT_F32>(pg, valid);
@@ -59,28 +60,29 @@ __device__ __forceinline__ void kept4(const GemmArgs& a, long long m, int n, f32
 // EPI_GATED_BWD: v is dh.
 template <int DT, int ACT, bool QUADS>
 __device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int n, f32x4 v, f32x4 g, f32x4 u) {
-    const int valid = a.N - n;
-    if (valid <= 0) return;
+    const int room = a.No - n, valid = a.N - n;
+    if (room <= 0) return;
     const long long c = (long long)n * ES<DT>;
     f32x4 dg, du, h;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float t, d;
         act_f<DT, ACT>(a.alpha, g[j], t, d);
-        dg[j] = v[j] * u[j] * d;
-        du[j] = v[j] * t;
+        const float w = j < valid ? v[j] : 0.0f;         // zeros behind the row's end, whatever the sum there was of
+        dg[j] = w * u[j] * d;
+        du[j] = w * t;
         h[j] = t * u[j];
     }
-    put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, dg, valid);
-    put4<DT, QUADS>(a.o[1] + m * a.ldo[1] + c, du, valid);
-    put4<DT, QUADS>(a.o[2] + m * a.ldo[2] + c, h, valid);
+    put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, dg, room);
+    put4<DT, QUADS>(a.o[1] + m * a.ldo[1] + c, du, room);
+    put4<DT, QUADS>(a.o[2] + m * a.ldo[2] + c, h, room);
 }
 
 // What becomes of four neighbouring sums of row m, columns n .. n+3 (v1: the second of EPI_GATED).
 template <int DT, int EPI, int ACT, bool QUADS>
 __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, int n, f32x4 v0, f32x4 v1) {
-    const int valid = a.N - n;
-    if (valid <= 0) return;
+    const int valid = a.N - n, room = a.No - n;
+    if (room <= 0) return;
     const long long c = (long long)n * ES<DT>, c4 = (long long)n * 4;
     if (EPI == EPI_STORE) {
         put4<DT, QUADS>((z ? a.o[1] : a.o[0]) + m * a.ldo[0] + c, v0, valid);
@@ -92,8 +94,8 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, 
             act_f<DT, ACT>(a.alpha, v0[j], t, d);
             h[j] = t * v1[j];
         }
-        put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, h, valid);
-        if (a.o[1]) {
+        put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, h, room);
+        if (a.o[1] && valid > 0) {
             put4<RT_F32, QUADS>(a.o[1] + m * a.ldo[1] + c4, v0, valid);
             put4<RT_F32, QUADS>(a.o[2] + m * a.ldo[2] + c4, v1, valid);
         }
@@ -248,7 +250,9 @@ struct Loader {
         const long long adv = L == LK ? k0 * ES<DT> : k0 * ld;
         if (AL) {
             // a tile spans less than 2^31 bytes (the host bounds ld), whatever the whole operand spans
-            const int span = L == LK ? (int)((rows - 1) * ld) + ke * ES<DT> : (int)((ke - 1) * ld) + rows * ES<DT>;
+            // (a row's last chunk is whole: it ends with the row, or with the zeros behind it)
+            const int whole = ((L == LK ? ke : rows) + EPC<DT> - 1) / EPC<DT> * 16;
+            const int span = (int)(((L == LK ? rows : ke) - 1) * ld) + whole;
             const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 #pragma unroll
             for (int it = 0; it < T::ITER; ++it) {

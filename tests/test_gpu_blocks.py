@@ -135,6 +135,15 @@ def test_gated_ffn_strides_and_alignment(engine, dt, lds, shift):
     ffn_case(engine, 5, 64, 128, 96, dt, "gelu", lds, shift, seed=6)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("size,lds,shift", [((1030, 101, 203, 77), (0, 0, 0, 0, 0), 0), ((1100, 36, 1001, 52), (0, 0, 0, 0, 0), 0),
+                                            ((1024, 64, 132, 33), (0, 0, 0, 0, 0), 0), ((1025, 43, 64, 65), (3, 1, 2, 5, 7), 1),
+                                            ((1500, 130, 66, 128), (6, 6, 0, 8, 2), 0), ((2050, 7, 5, 3), (0, 0, 0, 0, 0), 0)])
+def test_gated_ffn_odd_widths_of_many_rows(engine, size, lds, shift, dt):
+    """Operands that are copied with zeros behind their rows, beside ones that are not."""
+    ffn_case(engine, *size, dt, "sigmoid", lds, shift, seed=15, lo=dt != "f32")
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("size", [(1, 64, 128, 64), (2, 70, 256, 8), (3, 2000, 96, 5), (16, 128, 256, 128), (31, 72, 104, 40), (100, 130, 96, 66), (300, 512, 512, 64),
                                   (7, 33, 57, 31), (4100, 72, 4104, 16)], ids=lambda s: "x".join(map(str, s)))
