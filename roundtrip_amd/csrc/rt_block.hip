@@ -104,15 +104,14 @@ int check_ws(rt_ctx* ctx, const char* fn, const void* ws, size_t have, size_t ne
 // ---- matrix products ----------------------------------------------------------------------------------------------
 
 
-// Few rows against weights as they lie in memory: the weights' bytes are all the time there is.  Whether the kernel for
-// them can run depends on alignment too, so the workspace covers both.
-bool skinny_sizes(const Product& p) { return p.M <= SKINNY_ROWS && p.lx == LK && p.lw == LI && p.N % 4 == 0; }
+// Few rows against weights as they lie in memory: the weights' bytes are all the time there is.
+bool skinny_sizes(const Product& p) { return p.M <= SKINNY_ROWS && p.lx == LK && p.lw == LI && p.N >= 4; }
 
 void plan_skinny(int cus, int dtype, const Product& p, Plan& pl) {
     const int es = elem_size(dtype);
     pl.skinny = true;
     pl.nslot = p.epi == EPI_GATED ? 2 : 1;
-    pl.Np = p.N;
+    pl.Np = (int)up(p.N, 4);
     // Lanes of a row (gemv_kernel): 16 where that gives every CU a slab, or where there is so much to read that lines should
     // be read whole by one workgroup (32 MB: 6 us of the chip); else as few as give more workgroups.
     const int64_t all = p.K * p.N * es * pl.nslot;
@@ -185,7 +184,7 @@ int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, Ge
         a.quads = a.quads && (uintptr_t)a.o[i] % (4 * os) == 0 && a.ldo[i] % (4 * os) == 0;
     }
     if (p.epi == EPI_GATED_BWD) a.quads = a.quads && (uintptr_t)a.e[0] % 16 == 0 && (uintptr_t)a.e[1] % 16 == 0 && a.lde % 16 == 0;
-    if (skinny_sizes(p) && a.ldw[0] % (4 * es) == 0 && (uintptr_t)a.w[0] % (4 * es) == 0 && (uintptr_t)a.w[1] % (4 * es) == 0) {
+    if (skinny_sizes(p)) {
         plan_skinny(v.cu_count, dtype, p, pl);
         HIPCHK(ctx, dtype == RT_F32 ? launch_skinny<RT_F32>(v.stream, p, pl, a)
                     : dtype == RT_BF16 ? launch_skinny<RT_BF16>(v.stream, p, pl, a) : launch_skinny<RT_F16>(v.stream, p, pl, a));
@@ -231,13 +230,14 @@ constexpr int PAD_ROWS = 1024;
 // Raises `most` to the bytes of partial sums this product can need.
 int most_part_bytes(rt_ctx* ctx, int cus, int dtype, const Product& p, size_t& most) {
     Plan pl;
+    if (skinny_sizes(p)) {
+        plan_skinny(cus, dtype, p, pl);
+        if (pl.part_bytes > most) most = pl.part_bytes;
+        return RT_OK;
+    }
     for (int al = 0; al < 2; ++al) {
         const int rc = plan_product(ctx, cus, dtype, p, al, pl);
         if (rc) return rc;
-        if (pl.part_bytes > most) most = pl.part_bytes;
-    }
-    if (skinny_sizes(p)) {
-        plan_skinny(cus, dtype, p, pl);
         if (pl.part_bytes > most) most = pl.part_bytes;
     }
     return RT_OK;

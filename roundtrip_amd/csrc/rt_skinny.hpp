@@ -5,7 +5,7 @@
 //
 // Two kernels.  Both give a workgroup of 8 waves a slab of columns and all of K (or a split of it, where columns alone leave
 // the chip idle); lanes load four neighbouring columns of eight rows at a time, so that 64 lanes x eight loads are under way
-// before the first is needed; rows of X that do not exist are zeros, columns that do not exist are dropped.  The waves' sums
+// before the first is needed; rows of X that do not exist repeat the last and are dropped, like columns that do not exist.  The waves' sums
 // meet in LDS in a fixed order, the splits' in gemm_join_kernel.
 #pragma once
 #include "rt_gemm.hpp"
@@ -15,7 +15,9 @@
 template <int DT, int DUAL, int XR, int KS, bool LO>
 struct SkinnyStep {
     typedef typename Elem<DT>::T T;
-    struct __attribute__((aligned(4 * ES<DT>))) Four { T t[4]; };
+    struct Four { T t[4]; };
+    typedef unsigned Words __attribute__((ext_vector_type(ES<DT>)));
+    struct __attribute__((packed, aligned(2))) Loose { Words v; };       // four elements at the alignment of one
     Four w[DUAL][8];
     u32x4 x[XR][8 / EPC<DT>], lo[LO ? XR : 1];
 
@@ -29,12 +31,12 @@ struct SkinnyStep {
         for (int d = 0; d < DUAL; ++d)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const Four* p = (const Four*)((a.w[d] + (k0 + j) * ld) + at);
+                const Loose* p = (const Loose*)((a.w[d] + (k0 + j) * ld) + at);
                 if (whole) {
-                    w[d][j] = *p;
+                    w[d][j] = __builtin_bit_cast(Four, p->v);
                 } else {
                     w[d][j] = Four{};
-                    if (k + j < K) w[d][j] = *p;
+                    if (k + j < K) w[d][j] = __builtin_bit_cast(Four, p->v);
                 }
             }
 #pragma unroll
@@ -80,13 +82,17 @@ __device__ __forceinline__ void skinny_walk(int t, int steps, int stride, Load l
     }
 }
 
+// Where a quad of columns begins: the last one, if it is not whole, at N - 4 (its first columns are made twice, alike).
+__device__ __forceinline__ int quad_start(int n, int N) { return n < N - 4 ? n : N - 4; }
+
 // Four sums of row m, columns n ..: to the split's partial sums, or on to what becomes of them.
 template <int DT, int EPI>
 __device__ __forceinline__ void finish(const GemmArgs& a, int split, long long m, int n, const f32x4 (&v)[2]) {
     constexpr int DUAL = EPI == EPI_GATED ? 2 : 1;
     if (gridDim.y > 1) {
 #pragma unroll
-        for (int d = 0; d < DUAL; ++d) *(f32x4*)(a.part + (((long long)split * DUAL + d) * a.M + m) * a.Np + n) = v[d];
+        for (int d = 0; d < DUAL; ++d)
+            ((Chunk16*)(a.part + (((long long)split * DUAL + d) * a.M + m) * a.Np + n))->v = __builtin_bit_cast(u32x4, v[d]);
     } else {
         epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
             epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads>(a, 0, m, n, v[0], v[1]);
@@ -105,8 +111,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(GemmArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * SK_COLS, split = blockIdx.y, K = (int)a.K, steps = (K + 31) >> 5;
     const int stride = gridDim.y * NW;
-    // columns behind N: any that exist, they are dropped
-    const unsigned at = (unsigned)(8 * g * a.ldw[0]) + (unsigned)(n0 + 4 * i < a.N ? n0 + 4 * i : n0) * ES<DT>;
+    const unsigned at = (unsigned)(8 * g * a.ldw[0]) + (unsigned)quad_start(n0 + 4 * i, a.N) * ES<DT>;
 
     f32x4 acc[TILES][DUAL][4];
 #pragma unroll
@@ -171,7 +176,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(GemmArgs a) {
             for (int d = 0; d < DUAL; ++d)
 #pragma unroll
                 for (int w = 0; w < NW; ++w) v[d] += *(const f32x4*)sm[w][d][q][r];
-            finish<DT, EPI>(a, split, m, n, v);
+            finish<DT, EPI>(a, split, m, quad_start(n, a.N), v);
         }
     }
 }
@@ -189,7 +194,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void gemv_kernel(GemmArgs a) {
     const int tiles = gridDim.x, b = blockIdx.x, xcd = b & 7, r8 = tiles & 7;
     const int n0 = (xcd * (tiles >> 3) + (xcd < r8 ? xcd : r8) + (b >> 3)) * 4 * LI, split = blockIdx.y;
     const int K = (int)a.K, steps = (K + KS - 1) / KS, stride = gridDim.y * SK_WAVES;
-    const unsigned at = (unsigned)(8 * g * a.ldw[0]) + (unsigned)(n0 + 4 * i < a.N ? n0 + 4 * i : n0) * ES<DT>;
+    const unsigned at = (unsigned)(8 * g * a.ldw[0]) + (unsigned)quad_start(n0 + 4 * i, a.N) * ES<DT>;
 
     float acc[DUAL][MR][4];
 #pragma unroll
@@ -246,6 +251,6 @@ __global__ __launch_bounds__(64 * SK_WAVES) void gemv_kernel(GemmArgs a) {
         for (int d = 0; d < DUAL; ++d)
 #pragma unroll
             for (int w = 0; w < SK_WAVES; ++w) v[d] += *(const f32x4*)sm[w][d][m][q];
-        finish<DT, EPI>(a, split, m, n, v);
+        finish<DT, EPI>(a, split, m, quad_start(n, a.N), v);
     }
 }

@@ -152,6 +152,14 @@ def test_gated_ffn_with_the_rest_of_x(engine, size, dt):
     ffn_case(engine, *size, dt, "lrelu", seed=14, lo=True)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("size", [(1, 1501, 6293, 1502), (2, 70, 4, 5), (3, 35, 67, 131), (9, 100, 1023, 66), (32, 257, 5, 4), (4, 3000, 1030, 7)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_gated_ffn_few_rows_of_odd_widths(engine, size, dt):
+    ffn_case(engine, *size, dt, "gelu", seed=16)
+    ffn_case(engine, *size, dt, "gelu", (1, 3, 5, 7, 9), 1, seed=17)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_gated_ffn_long_sums(engine, dt):
     """Few columns under long sums: products whose K is split."""
