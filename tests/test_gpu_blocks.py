@@ -138,7 +138,7 @@ def test_gated_ffn_strides_and_alignment(engine, dt, lds, shift):
 @pytest.mark.parametrize("dt", ["bf16", "f32", "f16"])
 @pytest.mark.parametrize("size,lds,shift", [((1030, 101, 203, 77), (0, 0, 0, 0, 0), 0), ((1100, 36, 1001, 52), (0, 0, 0, 0, 0), 0),
                                             ((1024, 64, 132, 33), (0, 0, 0, 0, 0), 0), ((1025, 43, 64, 65), (3, 1, 2, 5, 7), 1),
-                                            ((1500, 130, 66, 128), (6, 6, 0, 8, 2), 0), ((2050, 7, 5, 3), (0, 0, 0, 0, 0), 0)])
+                                            ((1500, 130, 66, 128), (6, 6, 0, 8, 2), 0), ((1100, 130, 211, 33), (1, 0, 0, 0, 0), 0), ((2050, 7, 5, 3), (0, 0, 0, 0, 0), 0)])
 def test_gated_ffn_odd_widths_of_many_rows(engine, size, lds, shift, dt):
     """Operands that are copied with zeros behind their rows, beside ones that are not."""
     ffn_case(engine, *size, dt, "sigmoid", lds, shift, seed=15, lo=dt != "f32")
