@@ -164,7 +164,7 @@ int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Pla
             tn = n;
         }
     }
-    if (tm * tn > 0x7fffffff || steps > 0x7fffffff)
+    if (tm * tn > 0x7fffff || steps > 0x7fffffff)           // 512 threads a tile: a launch holds less than 2^32
         return failf(ctx, RT_EUNSUPPORTED, "a product of %lld x %d over %lld is larger than one launch covers", (long long)p.M, p.N,
                      (long long)p.K);
     pl.tiles_m = (int)tm;

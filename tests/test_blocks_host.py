@@ -185,3 +185,12 @@ def test_struct_layout_matches_the_header(tmp_path):
         assert int(got[n]) == C.sizeof(s)
         for f, _ in s._fields_:
             assert int(got["%s.%s" % (n, f)]) == getattr(s, f).offset, (n, f)
+
+
+def test_more_tiles_than_one_launch_holds_are_refused(lib):
+    """A launch holds less than 2^32 threads, a tile takes up to 512."""
+    a, n = ffn(T=1 << 34), C.c_size_t()
+    for backward in (0, 1):
+        refused(lib, lib.rt_gated_ffn_workspace(lib.ctx, C.byref(a), backward, C.byref(n)), EUNSUPPORTED, "one launch")
+    a = ffn(T=1 << 28)
+    assert lib.rt_gated_ffn_workspace(lib.ctx, C.byref(a), 0, C.byref(n)) == OK
