@@ -92,7 +92,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, 
         for (int j = 0; j < 4; ++j) {
             float t, d;
             act_f<DT, ACT>(a.alpha, v0[j], t, d);
-            h[j] = t * v1[j];
+            h[j] = j < valid ? t * v1[j] : 0.0f;          // behind the row's end zeros, where an infinite x left NaN too
         }
         put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, h, room);
         if (a.o[1] && valid > 0) {

@@ -616,3 +616,28 @@ def test_block_norm_without_tokens(engine):
     engine.sync()
     for t in w:
         assert not t.view.any() and t.untouched_outside()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_gated_ffn_infinities_stay_in_their_rows(engine, dt):
+    """Positive weights: an infinite x makes an infinite output row, with and without operands padded by zeros."""
+    T, di, f, do = 1030, 13, 21, 11
+    gen = torch.Generator().manual_seed(3)
+    x = (torch.rand((T, di), generator=gen) + 0.5).to(DT[dt])
+    x[7, 4] = float("inf")
+    w = [(torch.rand(s, generator=gen) + 0.5).to(DT[dt]) for s in ((di, f), (di, f), (f, do))]
+    want = ref.ffn(x.double(), w[0].double(), w[1].double(), w[2].double(), "silu", 0.0, DT[dt])
+    rows = [r for r in range(T) if r != 7]
+    ax, ag, au, ad = [Array(t.shape[0], t.shape[1], DT[dt], None, 0, t) for t in [x] + w]
+    for n_rows in (T, 20):
+        ao = Array(n_rows, do, DT[dt])
+        a = engine.gated_ffn_args(n_rows, di, f, do, CODE[dt], ACT["silu"], x=ax.ptr, w_gate=ag.ptr, w_up=au.ptr, w_down=ad.ptr, out=ao.ptr)
+        n = engine.gated_ffn_workspace(a)
+        ws = workspace(n)
+        torch.cuda.synchronize()
+        engine.gated_ffn_dev(a, ws.data_ptr(), n)
+        engine.sync()
+        assert bool((ao.view[7] == float("inf")).all())
+        keep = [r for r in rows if r < n_rows]
+        out = want["out"]
+        ref.check(ao.view[keep], tuple(t[keep] for t in out), "out")
