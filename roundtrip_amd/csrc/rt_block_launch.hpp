@@ -45,7 +45,9 @@ hipError_t launch_join(hipStream_t st, GemmFn join, int64_t M, int Np, int nbatc
 template <int DT, bool AL, int TPR, int NV>
 void launch_norm_fwd(hipStream_t st, const NormArgs& a) {
     constexpr int B = norm_block(TPR), RPB = B / TPR;
-    hipLaunchKernelGGL((norm_kernel<DT, TPR, NV, AL>), dim3((unsigned)((a.T + RPB - 1) / RPB)), dim3(B), 0, st, a);
+    // a launch holds less than 2^32 threads in x: more rows go on in y
+    const int64_t n = (a.T + RPB - 1) / RPB, x = n < (1 << 21) ? n : 1 << 21;
+    hipLaunchKernelGGL((norm_kernel<DT, TPR, NV, AL>), dim3((unsigned)x, (unsigned)((n + x - 1) / x)), dim3(B), 0, st, a);
 }
 
 template <int DT, bool AL, int TPR, int NV>
@@ -60,7 +62,7 @@ void pick_norm(hipStream_t st, const NormArgs& a, int tpr, bool back) {
         constexpr int PER = DT == RT_F32 ? 2 : 1;
         if (tpr == 64) nv <= 1 ? launch_norm_back<DT, AL, 64, 1>(st, a) : launch_norm_back<DT, AL, 64, PER>(st, a);
         else if (tpr == 256) nv <= 1 ? launch_norm_back<DT, AL, 256, 1>(st, a) : launch_norm_back<DT, AL, 256, PER>(st, a);
-        else if (tpr == 512) nv <= 1 ? launch_norm_back<DT, AL, 512, 1>(st, a) : launch_norm_back<DT, AL, 512, 2>(st, a);
+        else if (tpr == 512) nv <= PER ? launch_norm_back<DT, AL, 512, PER>(st, a) : launch_norm_back<DT, AL, 512, 2>(st, a);
         else if (nv <= 2) launch_norm_back<DT, AL, 1024, 2>(st, a);
         else launch_norm_back<DT, AL, 1024, 4>(st, a);
     } else if (tpr == 64) {

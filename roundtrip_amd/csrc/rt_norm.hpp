@@ -158,7 +158,7 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
     const int t = threadIdx.x % TPR;
     constexpr int WAVES = norm_block(TPR) / TPR;
     const int w = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
-    const long long row = (long long)blockIdx.x * WAVES + w;
+    const long long row = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * WAVES + w;
     if (row >= a.T) return;                     // TPR > 64: the whole workgroup (one row); else the whole wave
     const float inv = 1.0f / (float)a.d;
     M mx, mb, mg, mpost, mpre;

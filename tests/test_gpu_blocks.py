@@ -641,3 +641,19 @@ def test_gated_ffn_infinities_stay_in_their_rows(engine, dt):
         keep = [r for r in rows if r < n_rows]
         out = want["out"]
         ref.check(ao.view[keep], tuple(t[keep] for t in out), "out")
+
+
+@pytest.mark.parametrize("T,d", [((1 << 26) + 5, 8), ((1 << 21) * 4 + 3, 520)])
+def test_block_norm_of_more_rows_than_one_row_of_workgroups(engine, T, d):
+    x = torch.empty((T, d), dtype=torch.bfloat16, device="cuda")
+    x.random_(-4, 5, generator=torch.Generator(device="cuda").manual_seed(2))
+    n = torch.full_like(x, GUARD)
+    a = engine.block_norm_args(T, d, _lib.RT_BF16, _lib.RT_NORM_RMS, x=x.data_ptr(), n=n.data_ptr(), eps=0.25)
+    torch.cuda.synchronize()
+    engine.block_norm_dev(a)
+    engine.sync()
+    for r0 in (0, (1 << 23) - 50, T // 2, T - 100):
+        v = x[r0:r0 + 100].double()
+        want = v / (v.square().mean(1, keepdim=True) + 0.25).sqrt()
+        # half a step of bf16, and some float32 roundings
+        assert bool(((n[r0:r0 + 100].double() - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -20)).all())
