@@ -240,7 +240,10 @@ __global__ __launch_bounds__(64 * NW) void is_fused_kernel(const IsArgs a) {
             }
             return r;
         };
-        if (!left && n_u != n_loaded) {
+        // The same for the whole workgroup, and said so: as a branch that masks lanes the register allocator has put a copy of a
+        // value for phase D (lane * rem) behind it where the lanes were still off, and every query point of a leftover pass got
+        // the first one's score.
+        if (__builtin_amdgcn_readfirstlane(!left && n_u != n_loaded)) {
             // the previous pass's readers of yb / xh are past the barrier that ends its scoring phase
             for (int d = tid; d < dy; d += NTHREADS) yb[d] = a.y[n_u * dy + d];
             for (int d = tid; d < dx; d += NTHREADS) xh[d] = a.xhat[n_u * dx + d];
