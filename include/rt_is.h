@@ -336,7 +336,8 @@ typedef struct rt_gated_ffn_grads {
 } rt_gated_ffn_grads;
 
 /* Bytes of workspace rt_gated_ffn_dev (backward = 0) or rt_gated_ffn_backward_dev (1) needs for these sizes (pointers and
- * strides are not looked at): T x d_ff values, three times that backward, and the partial sums of products whose K is split. */
+ * strides are not looked at): T x d_ff values, three times that backward, the partial sums of products whose K is split, and,
+ * from 1024 rows on, copies of the operands whose widths are no multiples of 16 bytes. */
 int rt_gated_ffn_workspace(rt_ctx* ctx, const rt_gated_ffn* args, int backward, size_t* bytes);
 
 /* Forward.  h is rounded to the call's dtype on its way into the second product, as every operand of a matrix instruction is. */

@@ -6,6 +6,9 @@
 // Bound by memory: a row is read once and held in registers (TPR threads a row, NV 16-byte chunks a thread) while its
 // sums are made in float32, and every output is written once.  What limits short calls is the chain load - sum - load: all
 // of a row's arrays are asked for before the first is used, and sums that do not wait for each other share one exchange.
+//
+// Measured: 16384 x 4096 bf16 with branch and gate 97 us = 5.5 TB/s (a large copy: 5.2); one row 4.1 us, of which about 4 are
+// the launch.  A wave a row up to 256 chunks, where there are rows enough: no barrier in the chain.
 #pragma once
 #include "rt_elem.hpp"
 
@@ -217,6 +220,10 @@ __device__ __forceinline__ int gate_slot(long long group, long long unit_row0, l
 // (`together`) and their sums meet in LDS at its end; where short, a wave takes whole segments.  A segment's sum goes to
 // dgate if the unit saw all of the gate's rows, else to one of the unit's two partial slots.
 //
+// Measured: 8191 x 4096 bf16, gates of 1000 rows, 97 us for 403 MB = 4.1 TB/s and the join 9; 10000 x 512 float32 28 us = 4.4
+// TB/s and 5.  Two arrays of loads in turn (even, odd) with rows' bounds in the buffers instead of branches: 186 -> 52 us for
+// the float32 training step, 239 -> 145 for the bf16 one, of which the forward pass has 20 and 51.
+//
 //   t = dy + dN(dn w_pre at y);  dx = rs t;  q = bs t;  db = dN(q gate w_post at b)
 //   dN(z at v) = r (z - vh mean(z vh) [- mean z]),  vh = r v',  r = 1 / sqrt(mean(v'^2) + eps)
 template <int DT, int TPR, int NV, bool AL>
@@ -399,7 +406,7 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_back_kernel(NormArgs a) 
 }
 
 // Column sums of the units' partial sums, in a fixed order: 32 columns x 32 row classes a workgroup, eight rows of a class under
-// way at a time.
+// way at a time.  Latency: 5 us for 500 units of 512 columns, 9 for 256 of 4096.
 // blockIdx.y + first: 0 post, 1 pre, 2 + g: gate group g (of those, only what more than one unit saw).
 template <int DT>
 __global__ __launch_bounds__(1024) void norm_join_kernel(NormArgs a, int first) {
