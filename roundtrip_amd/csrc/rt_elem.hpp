@@ -21,6 +21,15 @@ template <> struct Elem<RT_F16> { typedef _Float16 T; typedef f16x4 Quad; };
 template <int DT> constexpr int ES = (int)sizeof(typename Elem<DT>::T);
 template <int DT> constexpr int EPC = 16 / ES<DT>;          // elements in a 16-byte chunk
 
+// v rounded to the type, from the float32 that it is.  float16: the compiler may fold a product before it into an instruction that
+// rounds once instead (v_fma_mixlo_f16), here and not there; one value in 16000 would then depend on which store a call's
+// alignment gives it, and differ from what n_lo is the rest of.
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::T to_elem(float v) {
+    if (DT == RT_F16) asm("" : "+v"(v));
+    return (typename Elem<DT>::T)v;
+}
+
 // `valid` of the EPC elements at p, zeros behind them.  AL: p is 16-byte aligned and a chunk is all valid or not at all.
 template <int DT, bool AL>
 __device__ __forceinline__ u32x4 load_chunk(const void* p, int valid) {
@@ -69,12 +78,12 @@ __device__ __forceinline__ void store_chunk(void* p, const float (&v)[EPC<DT>], 
     if (valid >= EPC<DT>) {
         union { T t[EPC<DT>]; u32x4 c; } u;
 #pragma unroll
-        for (int e = 0; e < EPC<DT>; ++e) u.t[e] = (T)v[e];
+        for (int e = 0; e < EPC<DT>; ++e) u.t[e] = to_elem<DT>(v[e]);
         if (AL) *(u32x4*)p = u.c; else ((Chunk16*)p)->v = u.c;
     } else {
 #pragma unroll
         for (int e = 0; e < EPC<DT>; ++e)
-            if (e < valid) ((T*)p)[e] = (T)v[e];
+            if (e < valid) ((T*)p)[e] = to_elem<DT>(v[e]);
     }
 }
 
@@ -85,12 +94,12 @@ __device__ __forceinline__ void store4(void* p, f32x4 v, int valid) {
     if (valid >= 4) {
         union { T t[4]; u32x4 c; unsigned long long h; } u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u.t[e] = (T)v[e];
+        for (int e = 0; e < 4; ++e) u.t[e] = to_elem<DT>(v[e]);
         if (ES<DT> == 4) ((Chunk16*)p)->v = u.c; else ((Chunk8*)p)->v = u.h;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (e < valid) ((T*)p)[e] = (T)v[e];
+            if (e < valid) ((T*)p)[e] = to_elem<DT>(v[e]);
     }
 }
 

@@ -46,7 +46,7 @@ template <int DT, bool QUADS>
 __device__ __forceinline__ void put4(char* p, f32x4 v, int valid) {
     typedef typename Elem<DT>::T T;
     typedef T T4 __attribute__((ext_vector_type(4)));
-    if (QUADS) *(T4*)p = T4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    if (QUADS) *(T4*)p = T4{to_elem<DT>(v[0]), to_elem<DT>(v[1]), to_elem<DT>(v[2]), to_elem<DT>(v[3])};
     else store4<DT>(p, v, valid);
 }
 

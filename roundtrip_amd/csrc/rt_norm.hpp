@@ -114,7 +114,7 @@ struct Row {
             if (AL) {
                 union { T t[E]; u32x4 c; } u;
 #pragma unroll
-                for (int e = 0; e < E; ++e) u.t[e] = (T)v[k][e];
+                for (int e = 0; e < E; ++e) u.t[e] = to_elem<DT>(v[k][e]);
                 __builtin_amdgcn_raw_buffer_store_b128(u.c, r, at * ES<DT>, 0, 0);
             } else if (p && at < d) {
                 store_chunk<DT, AL>(p + (unsigned)at * (unsigned)ES<DT>, v[k], d - at);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
         if (a.w_pre) v.times(R(mpre), a.w_off);
         v.store(a.n + row * a.ldn, a.d, t);
         if (a.n_lo) {                            // what the rounding left off
-            FOR_ROW(k, e) v.v[k][e] -= (float)(typename Elem<DT>::T)v.v[k][e];
+            FOR_ROW(k, e) v.v[k][e] -= (float)to_elem<DT>(v.v[k][e]);
             v.store(a.n_lo + row * a.ldn, a.d, t);
         }
     }
@@ -446,6 +446,6 @@ __global__ __launch_bounds__(1024) void norm_join_kernel(NormArgs a, int first) 
         float v = 0.0f;
 #pragma unroll
         for (int k = 0; k < RC; ++k) v += sm[k][threadIdx.x & 31];
-        ((T*)out)[c] = (T)v;
+        ((T*)out)[c] = to_elem<DT>(v);
     }
 }
