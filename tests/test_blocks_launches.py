@@ -1,4 +1,5 @@
 """Which kernels the network-block operators launch, seen without a GPU (launches.py)."""
+import ctypes as C
 import os
 
 import pytest
@@ -126,3 +127,35 @@ def test_sizes_of_the_measured_figures_get_the_kernels_named_there(double):
     assert names(fwd) == ["gemm_kernel<0, 0, 1, 1, 128, 128, 2, 2, true>", "gemm_kernel<0, 0, 1, 0, 64, 64, 2, 2, true>"]
     fwd, _ = double.ffn(1, 4096, 16384, 4096, "bf16")
     assert names(fwd) == ["gemv_kernel<1, 1, 1, 16, false>", "gemv_kernel<1, 0, 1, 16, false>", "gemm_join_kernel<1, 0>"]
+
+
+def every_entry(double):
+    """(name, a call that launches) of each entry point."""
+    f, r = double.ffn_args(40, 64, 96, 32, "bf16")
+    n, s = double.norm_args(20, 64, "f32", "rms", 3)
+    L, ws = double.lib, (double.WS, 1 << 62)
+    return [("rt_gated_ffn_dev", lambda: L.rt_gated_ffn_dev(double.ctx, C.byref(f), *ws)),
+            ("rt_gated_ffn_backward_dev", lambda: L.rt_gated_ffn_backward_dev(double.ctx, C.byref(f), C.byref(r), *ws)),
+            ("rt_block_norm_dev", lambda: L.rt_block_norm_dev(double.ctx, C.byref(n))),
+            ("rt_block_norm_backward_dev", lambda: L.rt_block_norm_backward_dev(double.ctx, C.byref(n), C.byref(s), *ws))]
+
+
+def test_the_current_device_stays_current(double):
+    """A context of another device than the current one: its device is current for the launches, the other one again behind
+    them, also where one fails half-way."""
+    other = launches.Double(device=3)
+    for name, call in every_entry(other):
+        other.reset(current=1)
+        assert call() == 0, name
+        lines = other.calls()
+        assert lines[0] == "device 3" and lines[-1] == "device 1", (name, lines)
+        assert len(lines) > 2 and all(line.endswith("on device 3") for line in lines[1:-1]), (name, lines)
+        for fail_at in range(len(lines) - 2):
+            other.reset(current=1, fail_at=fail_at)
+            assert call() == 2 and "an error of the double" in other.error(), (name, fail_at)       # RT_EHIP
+            assert other.lib.double_current() == 1, (name, fail_at)
+            assert len(other.calls()) == fail_at + 3, (name, fail_at)      # and nothing is launched behind the one that failed
+    for name, call in every_entry(double):
+        double.reset(current=0)
+        assert call() == 0
+        assert not [line for line in double.calls() if line.startswith("device")], name
