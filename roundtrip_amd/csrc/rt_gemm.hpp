@@ -33,7 +33,9 @@ __device__ __forceinline__ void act_f(float alpha, float g, float& a, float& d) 
         const float c2 = 1.5957691216057308f, c3 = 0.044715f;      // 2 sqrt(2 / pi)
         const float s = sigmoid_f<DT>(c2 * (g + c3 * g * g * g));
         a = g * s;
-        d = s + a * (1.0f - s) * c2 * (1.0f + 3.0f * c3 * g * g);
+        // from |g| = 64 on s (1 - s) is 0, and g^2 would not be finite for all g
+        const float b = __builtin_amdgcn_fmed3f(g, -64.0f, 64.0f);
+        d = s + b * s * (1.0f - s) * c2 * (1.0f + 3.0f * c3 * b * b);
     } else {
         const float s = sigmoid_f<DT>(g);
         a = ACT == RT_ACT_SILU ? g * s : s;

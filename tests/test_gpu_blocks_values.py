@@ -2,6 +2,7 @@
 import pytest
 
 torch = pytest.importorskip("torch")
+import block_ref as ref  # noqa: E402
 from test_gpu_blocks import ACT, CODE, DT, norm_case, workspace  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +37,29 @@ def test_bits_do_not_depend_on_what_is_kept_nor_where(engine, act, dt):
 def test_n_and_its_rest_of_many_values(engine, d, dt):
     """n + n_lo at two million values: one whose n was rounded otherwise than n_lo supposes would be off by a step of n."""
     norm_case(engine, 4096, d, dt, "rms", 0, branch=False, want_y=False, seed=d)
+
+
+@pytest.mark.parametrize("act", sorted(ACT))
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_gradient_of_large_gates(engine, act, dt):
+    """act'(g) for gates up to the type's end: with unit weights and ones for up and dout, dx is act'(g), rounded once in 16 bits
+    (dg; the sum over k then adds zeros)."""
+    dtype = DT[dt]
+    g = torch.tensor([0.0, 1.0, -1.0, 6.0, -6.0, 30.0, -30.0, 70.0, -70.0, 1e4, -1e4, 8e12, -8e12, 1.9e19, -1.9e19, 3e38, -3e38])
+    f = g.numel()
+    T = 3
+    eye, zero = torch.eye(f, dtype=dtype, device="cuda"), torch.zeros(f, f, dtype=dtype, device="cuda")
+    x, dout, dx = (torch.ones(T, f, dtype=dtype, device="cuda") for _ in range(3))
+    pg, pu = g.expand(T, f).contiguous().cuda(), torch.ones(T, f, device="cuda")
+    a = engine.gated_ffn_args(T, f, f, f, CODE[dt], ACT[act], x=x.data_ptr(), w_gate=eye.data_ptr(), w_up=zero.data_ptr(), w_down=eye.data_ptr(),
+                              out=x.data_ptr(), pre_gate=pg.data_ptr(), pre_up=pu.data_ptr(), alpha=0.25)
+    n = engine.gated_ffn_workspace(a, backward=True)
+    ws = workspace(n)
+    torch.cuda.synchronize()
+    engine.gated_ffn_backward_dev(a, engine.gated_ffn_grads(dout=dout.data_ptr(), dx=dx.data_ptr()), ws.data_ptr(), n)
+    engine.sync()
+    d = ref.act(act, g.double(), 0.25)[1].expand(T, f)
+    # float32's: ref.ACT where exp's argument is up to 16 in size; at the tails of exp (30 and beyond) the derivative is below 1e-11 or
+    # that near 1
+    tail = (2 * ref.ACT[dtype] * (d.abs() + g.double().abs().clamp(max=16)) + 1e-11).expand(T, f)
+    ref.check(dx, ref.rounded(d, tail, dtype), "dx")
