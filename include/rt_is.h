@@ -366,7 +366,8 @@ typedef struct rt_block_norm {
     const void *w_post, *w_pre;  /* d or NULL */
     void *y, *n;                 /* T x d; one of them may be NULL; each may be x's or branch's own memory, row for row */
     void *n_lo;                  /* 16-bit types: T x d with n's stride, or NULL: what n's rounding left off, so that n + n_lo has
-                                    twice the digits.  A gate's sign hangs on them: leaky ReLU's slope jumps at 0. */
+                                    twice the digits (0 where n is infinite).  A gate's sign hangs on them: leaky
+                                    ReLU's slope jumps at 0. */
 } rt_block_norm;
 
 /* Gradients of sum(dy * y) + sum(dn * n).  dy or dn may be NULL (zeros); a NULL output is not computed. */

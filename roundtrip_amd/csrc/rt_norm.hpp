@@ -202,8 +202,11 @@ __global__ __launch_bounds__(norm_block(TPR)) void norm_kernel(NormArgs a) {
         v.scale(f);
         if (a.w_pre) v.times(R(mpre), a.w_off);
         v.store(a.n + row * a.ldn, a.d, t);
-        if (a.n_lo) {                            // what the rounding left off
-            FOR_ROW(k, e) v.v[k][e] -= (float)to_elem<DT>(v.v[k][e]);
+        if (a.n_lo) {                            // what the rounding left off: nothing of what it made infinite
+            FOR_ROW(k, e) {
+                const float r = (float)to_elem<DT>(v.v[k][e]);
+                v.v[k][e] = __builtin_isinf(r) ? 0.0f : v.v[k][e] - r;
+            }
             v.store(a.n_lo + row * a.ldn, a.d, t);
         }
     }

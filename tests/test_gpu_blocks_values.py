@@ -3,7 +3,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 import block_ref as ref  # noqa: E402
-from test_gpu_blocks import ACT, CODE, DT, norm_case, workspace  # noqa: E402
+from roundtrip_amd import _lib  # noqa: E402
+from test_gpu_blocks import ACT, CODE, DT, KIND, norm_case, workspace  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,47 @@ def test_gradient_of_large_gates(engine, act, dt):
     # that near 1
     tail = (2 * ref.ACT[dtype] * (d.abs() + g.double().abs().clamp(max=16)) + 1e-11).expand(T, f)
     ref.check(dx, ref.rounded(d, tail, dtype), "dx")
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("dt,w", [("f16", 6e4), ("bf16", 3e38)])
+def test_the_rest_of_an_infinite_value_is_zero(engine, dt, w, kind):
+    """Normed rows beyond the type's range are infinite, and n_lo is zero there: n + n_lo, and a product with positive weights,
+    are infinite and not NaN."""
+    T, d, f = 40, 64, 72
+    dtype = DT[dt]
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(T, d, generator=gen).to(dtype)
+    x64 = x.double()
+    c = x64 - x64.mean(1, keepdim=True) if kind == "layer" else x64
+    hat = c / (c.square().mean(1, keepdim=True) + 1e-5).sqrt()
+    wp = torch.ones(d, dtype=dtype)
+    wp[5] = w
+    beyond = torch.zeros(T, d, dtype=torch.bool)
+    beyond[:, 5] = hat[:, 5].abs() > 1.3                 # 1.3 w is beyond either type by more than the norm's error
+    near = torch.zeros(T, d, dtype=torch.bool)
+    near[:, 5] = (hat[:, 5].abs() > 1.0) & ~beyond[:, 5]
+    assert 3 < int(beyond.sum()) < T - 3
+    dev = [t.cuda() for t in (x, wp)]
+    n, lo = torch.empty_like(dev[0]), torch.empty_like(dev[0])
+    a = engine.block_norm_args(T, d, CODE[dt], KIND[kind], x=dev[0].data_ptr(), n=n.data_ptr(), n_lo=lo.data_ptr(), w_pre=dev[1].data_ptr(), eps=1e-5)
+    torch.cuda.synchronize()
+    engine.block_norm_dev(a)
+    engine.sync()
+    got, rest = n.cpu().double(), lo.cpu().double()
+    assert torch.equal(got[beyond], torch.sign(hat[beyond]) * float("inf"))
+    assert not rest[beyond].any()
+    fine = ~beyond & ~near
+    assert torch.isfinite(got[fine]).all() and torch.isfinite(rest[fine]).all()
+    # the block behind it: positive weights, so that gate and up are +infinity where x is
+    ones = [torch.full(s, 2.0 ** -4, dtype=dtype, device="cuda") for s in ((d, f), (d, f), (f, d))]
+    out = torch.empty(T, d, dtype=dtype, device="cuda")
+    b = engine.gated_ffn_args(T, d, f, d, CODE[dt], ACT["silu"], x=n.data_ptr(), x_lo=lo.data_ptr(), w_gate=ones[0].data_ptr(), w_up=ones[1].data_ptr(),
+                              w_down=ones[2].data_ptr(), out=out.data_ptr())
+    size = engine.gated_ffn_workspace(b)
+    ws = workspace(size)
+    torch.cuda.synchronize()
+    engine.gated_ffn_dev(b, ws.data_ptr(), size)
+    engine.sync()
+    rows = beyond[:, 5] & (hat[:, 5] > 0)
+    assert bool(rows.any()) and bool((out[rows.cuda()] == float("inf")).all())
