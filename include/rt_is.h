@@ -280,7 +280,7 @@ uint32_t rt_crc32c(const void* data, size_t n, uint32_t crc);
  * The layers deep networks put around and between plain dense ones, next to rt_mlp_forward_dev: a gated feed-forward block
  * and the norms before and after it, forward and backward.  NO COUNTERPART IN THE REFERENCE (its networks are chains of
  * dense layers, model.py:61-88).
- *   - all pointers in the structs are DEVICE pointers to arrays of the call's dtype (but for pre_gate, pre_up), rows contiguous; an ld* is the distance
+ *   - all pointers in the structs are DEVICE pointers to arrays of the call's dtype (pre_gate, pre_up: of pre_dtype), rows contiguous; an ld* is the distance
  *     of two rows in elements (0: rows are dense), at most 2^20.  Nothing needs more alignment than its elements have;
  *     arrays whose rows start on 16 bytes and are whole multiples of 16 bytes long are read fastest.
  *   - the sums of products, the norms' sums and everything between two stores are float32 or wider; a stored value is rounded
@@ -311,7 +311,9 @@ int rt_ctx_stream(rt_ctx* ctx, void** stream);
 
 /* out = h w_down,  h = act(x w_gate) * (x w_up)      T rows; widths and strides up to 2^20, T up to 2^40 */
 typedef struct rt_gated_ffn {
-    int32_t dtype, act;          /* RT_F32 / RT_BF16 / RT_F16;  RT_ACT_* */
+    int16_t dtype;               /* RT_F32 / RT_BF16 / RT_F16 */
+    int16_t pre_dtype;           /* of pre_gate and pre_up: RT_F32 (0) or dtype */
+    int32_t act;                 /* RT_ACT_* */
     int32_t d_in, d_ff, d_out;
     float   alpha;               /* RT_ACT_LRELU */
     int64_t T;                   /* 0: nothing to do (gradients of weights: zeros) */
@@ -322,8 +324,9 @@ typedef struct rt_gated_ffn {
     void *out;                   /* T x d_out */
     const void *x_lo;            /* 16-bit types: T x d_in with x's stride, or NULL: x + x_lo is what is multiplied by w_gate and
                                     w_up (rt_block_norm's n and n_lo); dw_gate and dw_up are of x alone */
-    float *pre_gate, *pre_up;    /* T x d_ff float32 in every dtype: x w_gate and x w_up, kept for the backward pass (rounded
-                                    to 16 bits they would double the error of every gradient); both NULL if there is none */
+    void *pre_gate, *pre_up;     /* T x d_ff of pre_dtype: x w_gate and x w_up, kept for the backward pass; both NULL if there is
+                                    none.  Float32 (four bytes an element) unless pre_dtype says otherwise, in every dtype:
+                                    rounded to 16 bits they take half the memory, and double the error of every gradient */
 } rt_gated_ffn;
 
 /* Gradients of sum(dout * out).  A NULL output is not computed. */

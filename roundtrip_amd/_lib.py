@@ -50,7 +50,7 @@ class RtCounters(C.Structure):
 class RtGatedFfn(C.Structure):
     """rt_gated_ffn (include/rt_is.h): one gated feed-forward block in device memory.  Kept by the caller and used as often
     as the addresses in it hold."""
-    _fields_ = ([(k, C.c_int32) for k in ("dtype", "act", "d_in", "d_ff", "d_out")] + [("alpha", C.c_float)]
+    _fields_ = ([(k, C.c_int16) for k in ("dtype", "pre_dtype")] + [(k, C.c_int32) for k in ("act", "d_in", "d_ff", "d_out")] + [("alpha", C.c_float)]
                 + [(k, C.c_int64) for k in ("T", "ldx", "ld_in", "ld_down", "ld_out", "ld_pre")]
                 + [(k, C.c_void_p) for k in ("x", "w_gate", "w_up", "w_down", "out", "x_lo", "pre_gate", "pre_up")])
 
@@ -397,9 +397,11 @@ class Engine(object):
 
     @staticmethod
     def gated_ffn_args(T, d_in, d_ff, d_out, dtype, act, x=None, w_gate=None, w_up=None, w_down=None, out=None,
-                       pre_gate=None, pre_up=None, x_lo=None, alpha=0.2, ldx=0, ld_in=0, ld_down=0, ld_out=0, ld_pre=0):
-        """out = (act(x w_gate) * (x w_up)) w_down; pre_gate / pre_up keep what the backward pass needs."""
-        return RtGatedFfn(dtype=dtype, act=act, d_in=d_in, d_ff=d_ff, d_out=d_out, alpha=alpha, T=T, ldx=ldx, ld_in=ld_in,
+                       pre_gate=None, pre_up=None, x_lo=None, alpha=0.2, ldx=0, ld_in=0, ld_down=0, ld_out=0, ld_pre=0,
+                       pre_dtype=RT_F32):
+        """out = (act(x w_gate) * (x w_up)) w_down; pre_gate / pre_up keep what the backward pass needs: float32 arrays, whatever
+        dtype is, or with pre_dtype=dtype arrays of that type."""
+        return RtGatedFfn(dtype=dtype, pre_dtype=pre_dtype, act=act, d_in=d_in, d_ff=d_ff, d_out=d_out, alpha=alpha, T=T, ldx=ldx, ld_in=ld_in,
                           ld_down=ld_down, ld_out=ld_out, ld_pre=ld_pre, x=x, w_gate=w_gate, w_up=w_up, w_down=w_down,
                           out=out, x_lo=x_lo, pre_gate=pre_gate, pre_up=pre_up)
 

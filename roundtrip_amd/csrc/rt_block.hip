@@ -176,14 +176,14 @@ int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Pla
 
 int run_product(rt_ctx* ctx, const RtCtxView& v, int dtype, const Product& p, GemmArgs& a) {
     Plan pl;
-    const int es = elem_size(dtype), epc = 16 / es;
+    const int es = elem_size(dtype), epc = 16 / es, kept = a.kept_narrow ? es : 4;
     a.quads = p.N % 4 == 0;
     for (int i = 0; i < 3; ++i) {
-        const int os = p.epi == EPI_GATED && i ? 4 : es;      // what the forward pass keeps is float32
+        const int os = p.epi == EPI_GATED && i ? kept : es;
         if (p.epi == EPI_STORE && i >= p.nrun) break;
         a.quads = a.quads && (uintptr_t)a.o[i] % (4 * os) == 0 && a.ldo[i] % (4 * os) == 0;
     }
-    if (p.epi == EPI_GATED_BWD) a.quads = a.quads && (uintptr_t)a.e[0] % 16 == 0 && (uintptr_t)a.e[1] % 16 == 0 && a.lde % 16 == 0;
+    if (p.epi == EPI_GATED_BWD) a.quads = a.quads && (uintptr_t)a.e[0] % (4 * kept) == 0 && (uintptr_t)a.e[1] % (4 * kept) == 0 && a.lde % (4 * kept) == 0;
     if (skinny_sizes(p)) {
         plan_skinny(v.cu_count, dtype, p, pl);
         HIPCHK(ctx, dtype == RT_F32 ? launch_skinny<RT_F32>(v.stream, p, pl, a)
@@ -215,7 +215,7 @@ int zero_rows(rt_ctx* ctx, hipStream_t st, void* p, int64_t ld, int64_t rows, in
 // ---- the gated feed-forward block ---------------------------------------------------------------------------------
 struct Ffn {
     rt_gated_ffn a;                // with its strides filled in
-    int es;
+    int es, kept;                  // bytes of an element; of the kept gate's and up's
     int64_t ldh;                   // elements; h, dgate and dup lie in the workspace
     size_t h_bytes;
     bool pad;                      // many rows: operands of odd widths are copied, padded
@@ -248,6 +248,8 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
     f.a = *in;
     rt_gated_ffn& a = f.a;
     if (a.dtype != RT_F32 && a.dtype != RT_BF16 && a.dtype != RT_F16) return failf(ctx, RT_EINVAL, "%s: unknown dtype %d", fn, a.dtype);
+    if (a.pre_dtype != RT_F32 && a.pre_dtype != a.dtype)
+        return failf(ctx, RT_EINVAL, "%s: pre_dtype %d is neither RT_F32 nor the arrays' type", fn, a.pre_dtype);
     if (a.act < RT_ACT_SILU || a.act > RT_ACT_SIGMOID) return failf(ctx, RT_EINVAL, "%s: unknown activation %d", fn, a.act);
     if (a.x_lo && a.dtype == RT_F32) return failf(ctx, RT_EINVAL, "%s: x_lo is for 16-bit types", fn);
     if (!isfinite(a.alpha)) return failf(ctx, RT_EINVAL, "%s: alpha is not finite", fn);
@@ -255,6 +257,7 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
     if (a.d_in < 1 || a.d_ff < 1 || a.d_out < 1 || a.d_in > MAX_DIM || a.d_ff > MAX_DIM || a.d_out > MAX_DIM)
         return failf(ctx, RT_EINVAL, "%s: widths %d, %d, %d: each must be in [1, %lld]", fn, a.d_in, a.d_ff, a.d_out, (long long)MAX_DIM);
     f.es = elem_size(a.dtype);
+    f.kept = elem_size(a.pre_dtype);
     if (!a.ldx) a.ldx = a.d_in;
     if (!a.ld_in) a.ld_in = a.d_ff;
     if (!a.ld_down) a.ld_down = a.d_out;
@@ -370,8 +373,9 @@ int ffn_forward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, char* ws) {
     set_x(g, o.x, a.x_lo ? o.x_lo : o.x, o.ldx);
     set_w(g, o.w_gate, o.w_up, o.ld_in);
     set_o(g, 0, h, f.ldh * es);
-    set_o(g, 1, a.pre_gate, a.ld_pre * 4);
-    set_o(g, 2, a.pre_up, a.ld_pre * 4);
+    set_o(g, 1, a.pre_gate, a.ld_pre * f.kept);
+    set_o(g, 2, a.pre_up, a.ld_pre * f.kept);
+    g.kept_narrow = f.kept < 4;
     if ((rc = run_product(ctx, v, a.dtype, f.gated, g))) return rc;
     set_x(g, h, h, f.ldh * es);
     set_w(g, o.w_down, o.w_down, o.ld_down);
@@ -399,7 +403,8 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
     set_o(g, 2, h, ldh);
     g.e[0] = (const char*)a.pre_gate;
     g.e[1] = (const char*)a.pre_up;
-    g.lde = a.ld_pre * 4;
+    g.lde = a.ld_pre * f.kept;
+    g.kept_narrow = f.kept < 4;
     if ((rc = run_product(ctx, v, a.dtype, f.dh, g))) return rc;
     if (r.dx) {                      // dx = dgate Wg^T + dup Wu^T: one sum over both
         set_x(g, dg, du, ldh);
@@ -546,8 +551,8 @@ int rt_gated_ffn_dev(rt_ctx* ctx, const rt_gated_ffn* args, void* ws, size_t ws_
     const rt_gated_ffn& a = f.a;
     const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx, f.es}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in, f.es}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in, f.es},
                       {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}, {"x_lo", a.x_lo, a.T, a.d_in, a.ldx, f.es}};
-    const Mat out[] = {{"out", a.out, a.T, a.d_out, a.ld_out, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, 4},
-                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, 4}, {"the workspace", ws, 1, (int64_t)f.ws_fwd, (int64_t)f.ws_fwd, 1}};
+    const Mat out[] = {{"out", a.out, a.T, a.d_out, a.ld_out, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, f.kept},
+                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, f.kept}, {"the workspace", ws, 1, (int64_t)f.ws_fwd, (int64_t)f.ws_fwd, 1}};
     for (int i = 0; i < 5; ++i)
         if ((rc = check_mat(ctx, fn, in[i], i < 4))) return rc;
     for (int i = 0; i < 3; ++i)
@@ -576,8 +581,8 @@ int rt_gated_ffn_backward_dev(rt_ctx* ctx, const rt_gated_ffn* args, const rt_ga
     if (!r.ld_dw_in) r.ld_dw_in = a.d_ff;
     if (!r.ld_dw_down) r.ld_dw_down = a.d_out;
     const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx, f.es}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in, f.es}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in, f.es},
-                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, 4},
-                      {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, 4}, {"dout", r.dout, a.T, a.d_out, r.ld_dout, f.es}};
+                      {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, f.kept},
+                      {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, f.kept}, {"dout", r.dout, a.T, a.d_out, r.ld_dout, f.es}};
     const Mat out[] = {{"dx", r.dx, a.T, a.d_in, r.ld_dx, f.es}, {"dw_gate", r.dw_gate, a.d_in, a.d_ff, r.ld_dw_in, f.es},
                        {"dw_up", r.dw_up, a.d_in, a.d_ff, r.ld_dw_in, f.es}, {"dw_down", r.dw_down, a.d_ff, a.d_out, r.ld_dw_down, f.es},
                        {"the workspace", ws, 1, (int64_t)f.ws_bwd, (int64_t)f.ws_bwd, 1}};

@@ -21,10 +21,11 @@ struct GemmArgs {
     float* part;                   // splits > 1: [split][slot][M][Np] partial sums, joined by gemm_join_kernel
     int Np, nslot;
     int No;                        // columns written: N, or more of the workspace's own rows, zeros that the next product may read
-    char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two float32 or NULL).
+    char* o[3];                    // EPI_STORE: o[blockIdx.z].  EPI_GATED: h, gate, up (the last two kept, or NULL).
     long long ldo[3];              // (EPI_STORE: ldo[0] for both)  EPI_GATED_BWD: dgate, dup, h
-    const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept, float32
+    const char* e[2];              // EPI_GATED_BWD: the gate and up that the forward pass kept
     long long lde;
+    int kept_narrow;               // what is kept has the call's type, not float32
     int act;
     float alpha;
     int quads;                     // N and every output's (and e's) place are multiples of four elements

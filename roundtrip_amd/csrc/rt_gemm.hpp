@@ -52,20 +52,35 @@ __device__ __forceinline__ void put4(char* p, f32x4 v, int valid) {
     else store4<DT>(p, v, valid);
 }
 
-// The kept gate and up at four places (columns behind N: nothing).
-template <bool QUADS>
-__device__ __forceinline__ void kept4(const GemmArgs& a, long long m, int n, f32x4& g, f32x4& u) {
+// Four kept values as they lie in memory, of type KT.
+template <int KT> struct Kept {
+    typedef typename Elem<KT>::Quad Quad;
+    Quad v;
+    template <bool QUADS> __device__ __forceinline__ void load(const char* p, int valid) {
+        if (QUADS) {
+            v = *(const Quad*)p;
+        } else {
+            const f32x4 f = load4<KT>(p, valid);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (typename Elem<KT>::T)f[j];       // from that type, so exact
+        }
+    }
+};
+
+// The kept gate and up at four places (columns behind N: zeros).
+template <int KT, bool QUADS>
+__device__ __forceinline__ void kept4(const GemmArgs& a, long long m, int n, Kept<KT>& g, Kept<KT>& u) {
     const int valid = a.N - n;
-    g = u = f32x4{0, 0, 0, 0};
+    g.v = u.v = typename Kept<KT>::Quad{0, 0, 0, 0};
     if (valid <= 0) return;
-    const char *pg = a.e[0] + m * a.lde + (long long)n * 4, *pu = a.e[1] + m * a.lde + (long long)n * 4;
-    g = QUADS ? *(const f32x4*)pg : load4<RT_F32>(pg, valid);
-    u = QUADS ? *(const f32x4*)pu : load4<RT_F32>(pu, valid);
+    const long long at = m * a.lde + (long long)n * ES<KT>;
+    g.template load<QUADS>(a.e[0] + at, valid);
+    u.template load<QUADS>(a.e[1] + at, valid);
 }
 
 // EPI_GATED_BWD: v is dh.
-template <int DT, int ACT, bool QUADS>
-__device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int n, f32x4 v, f32x4 g, f32x4 u) {
+template <int DT, int ACT, bool QUADS, int KT>
+__device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int n, f32x4 v, const Kept<KT>& kept_g, const Kept<KT>& kept_u) {
     const int room = a.No - n, valid = a.N - n;
     if (room <= 0) return;
     const long long c = (long long)n * ES<DT>;
@@ -73,11 +88,12 @@ __device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float t, d;
-        act_f<DT, ACT>(a.alpha, g[j], t, d);
+        const float u = (float)kept_u.v[j];
+        act_f<DT, ACT>(a.alpha, (float)kept_g.v[j], t, d);
         const float w = j < valid ? v[j] : 0.0f;         // zeros behind the row's end, whatever the sum there was of
-        dg[j] = w * u[j] * d;
+        dg[j] = w * u * d;
         du[j] = w * t;
-        h[j] = t * u[j];
+        h[j] = t * u;
     }
     put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, dg, room);
     put4<DT, QUADS>(a.o[1] + m * a.ldo[1] + c, du, room);
@@ -85,11 +101,11 @@ __device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int
 }
 
 // What becomes of four neighbouring sums of row m, columns n .. n+3 (v1: the second of EPI_GATED).
-template <int DT, int EPI, int ACT, bool QUADS>
+template <int DT, int EPI, int ACT, bool QUADS, int KT>
 __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, int n, f32x4 v0, f32x4 v1) {
     const int valid = a.N - n, room = a.No - n;
     if (room <= 0) return;
-    const long long c = (long long)n * ES<DT>, c4 = (long long)n * 4;
+    const long long c = (long long)n * ES<DT>, ck = (long long)n * ES<KT>;
     if (EPI == EPI_STORE) {
         put4<DT, QUADS>((z ? a.o[1] : a.o[0]) + m * a.ldo[0] + c, v0, valid);
     } else if (EPI == EPI_GATED) {
@@ -102,36 +118,39 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, long long m, 
         }
         put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, h, room);
         if (a.o[1] && valid > 0) {
-            put4<RT_F32, QUADS>(a.o[1] + m * a.ldo[1] + c4, v0, valid);
-            put4<RT_F32, QUADS>(a.o[2] + m * a.ldo[2] + c4, v1, valid);
+            put4<KT, QUADS>(a.o[1] + m * a.ldo[1] + ck, v0, valid);
+            put4<KT, QUADS>(a.o[2] + m * a.ldo[2] + ck, v1, valid);
         }
     } else {
-        f32x4 g, u;
-        kept4<QUADS>(a, m, n, g, u);
-        epilogue_bwd<DT, ACT, QUADS>(a, m, n, v0, g, u);
+        Kept<KT> g, u;
+        kept4<KT, QUADS>(a, m, n, g, u);
+        epilogue_bwd<DT, ACT, QUADS, KT>(a, m, n, v0, g, u);
     }
 }
 
-// body(ACT, QUADS) with both as constants: the choice is made once, outside the loops over a tile.
-template <int ACT, bool QUADS> struct EpiWay {
-    static constexpr int act = ACT;
+// body(ACT, QUADS, KT: the type of what is kept) with all as constants: the choice is made once, outside the loops over a tile.
+template <int ACT, bool QUADS, int KT> struct EpiWay {
+    static constexpr int act = ACT, kept = KT;
     static constexpr bool quads = QUADS;
 };
-template <int EPI, class Body>
+template <bool QUADS, int KT, class Body>
+__device__ __forceinline__ void epilogue_act(const GemmArgs& a, Body body) {
+    if (a.act == RT_ACT_SILU) body(EpiWay<RT_ACT_SILU, QUADS, KT>());
+    else if (a.act == RT_ACT_GELU_TANH) body(EpiWay<RT_ACT_GELU_TANH, QUADS, KT>());
+    else if (a.act == RT_ACT_LRELU) body(EpiWay<RT_ACT_LRELU, QUADS, KT>());
+    else body(EpiWay<RT_ACT_SIGMOID, QUADS, KT>());
+}
+template <int DT, int EPI, class Body>
 __device__ __forceinline__ void epilogue_way(const GemmArgs& a, Body body) {
     if (EPI == EPI_STORE) {
-        if (a.quads) body(EpiWay<0, true>());
-        else body(EpiWay<0, false>());
-    } else if (a.quads) {
-        if (a.act == RT_ACT_SILU) body(EpiWay<RT_ACT_SILU, true>());
-        else if (a.act == RT_ACT_GELU_TANH) body(EpiWay<RT_ACT_GELU_TANH, true>());
-        else if (a.act == RT_ACT_LRELU) body(EpiWay<RT_ACT_LRELU, true>());
-        else body(EpiWay<RT_ACT_SIGMOID, true>());
+        if (a.quads) body(EpiWay<0, true, RT_F32>());
+        else body(EpiWay<0, false, RT_F32>());
+    } else if (DT == RT_F32 || !a.kept_narrow) {
+        if (a.quads) epilogue_act<true, RT_F32>(a, body);
+        else epilogue_act<false, RT_F32>(a, body);
     } else {
-        if (a.act == RT_ACT_SILU) body(EpiWay<RT_ACT_SILU, false>());
-        else if (a.act == RT_ACT_GELU_TANH) body(EpiWay<RT_ACT_GELU_TANH, false>());
-        else if (a.act == RT_ACT_LRELU) body(EpiWay<RT_ACT_LRELU, false>());
-        else body(EpiWay<RT_ACT_SIGMOID, false>());
+        if (a.quads) epilogue_act<true, DT>(a, body);
+        else epilogue_act<false, DT>(a, body);
     }
 }
 
@@ -413,16 +432,16 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& a, int z, int split,
         }
         return;
     }
-    epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
-        constexpr int ACT = decltype(way)::act;
+    epilogue_way<DT, EPI>(a, [&](auto way) __attribute__((always_inline)) {
+        constexpr int ACT = decltype(way)::act, KT = decltype(way)::kept;
         constexpr bool QUADS = decltype(way)::quads;
         if constexpr (EPI == EPI_GATED_BWD) {            // what it reads is asked for a row of tiles ahead
-            f32x4 gate[2][H], up[2][H];
+            Kept<KT> gate[2][H], up[2][H];
             auto ask = [&](int mt) __attribute__((always_inline)) {
                 const long long m = m0 + mt * 16 + i;
 #pragma unroll
                 for (int j = 0; j < H; ++j)
-                    if (m < a.M) kept4<QUADS>(a, m, n0 + j * 16 + 4 * g, gate[mt & 1][j], up[mt & 1][j]);
+                    if (m < a.M) kept4<KT, QUADS>(a, m, n0 + j * 16 + 4 * g, gate[mt & 1][j], up[mt & 1][j]);
             };
             ask(0);
 #pragma unroll
@@ -432,7 +451,7 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& a, int z, int split,
                 if (m >= a.M) continue;
 #pragma unroll
                 for (int j = 0; j < H; ++j)
-                    epilogue_bwd<DT, ACT, QUADS>(a, m, n0 + j * 16 + 4 * g, acc[mt][j], gate[mt & 1][j], up[mt & 1][j]);
+                    epilogue_bwd<DT, ACT, QUADS, KT>(a, m, n0 + j * 16 + 4 * g, acc[mt][j], gate[mt & 1][j], up[mt & 1][j]);
             }
         } else {
 #pragma unroll
@@ -441,7 +460,7 @@ __device__ __forceinline__ void finish_tile(const GemmArgs& a, int z, int split,
                 if (m >= a.M) continue;
 #pragma unroll
                 for (int j = 0; j < H; ++j)
-                    epilogue<DT, EPI, ACT, QUADS>(a, z, m, n0 + j * 16 + 4 * g, acc[mt][j], acc[mt][DUAL == 2 ? j + H : j]);
+                    epilogue<DT, EPI, ACT, QUADS, KT>(a, z, m, n0 + j * 16 + 4 * g, acc[mt][j], acc[mt][DUAL == 2 ? j + H : j]);
             }
         }
     });
@@ -641,8 +660,8 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
                 for (int d = 0; d < DUAL; ++d)
                     if (s + b < a.splits) v[d] += t[b][d];
         }
-        epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
-            epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads>(a, z, m, n, v[0], v[1]);
+        epilogue_way<DT, EPI>(a, [&](auto way) __attribute__((always_inline)) {
+            epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads, decltype(way)::kept>(a, z, m, n, v[0], v[1]);
         });
     }
 }

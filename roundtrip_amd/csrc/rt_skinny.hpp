@@ -97,8 +97,8 @@ __device__ __forceinline__ void finish(const GemmArgs& a, int split, long long m
         for (int d = 0; d < DUAL; ++d)
             ((Chunk16*)(a.part + (((long long)split * DUAL + d) * a.M + m) * a.Np + n))->v = __builtin_bit_cast(u32x4, v[d]);
     } else {
-        epilogue_way<EPI>(a, [&](auto way) __attribute__((always_inline)) {
-            epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads>(a, 0, m, n, v[0], v[1]);
+        epilogue_way<DT, EPI>(a, [&](auto way) __attribute__((always_inline)) {
+            epilogue<DT, EPI, decltype(way)::act, decltype(way)::quads, decltype(way)::kept>(a, 0, m, n, v[0], v[1]);
         });
     }
 }
