@@ -309,7 +309,9 @@ uint32_t rt_crc32c(const void* data, size_t n, uint32_t crc);
  * into a graph.  It stays the context's: do not destroy it. */
 int rt_ctx_stream(rt_ctx* ctx, void** stream);
 
-/* out = h w_down,  h = act(x w_gate) * (x w_up)      T rows; widths and strides up to 2^20, T up to 2^40 */
+/* out = h w_down,  h = act(x w_gate) * (x w_up)      T rows; widths and strides up to 2^20.  A product may have up to 2^23 - 1
+ * tiles of 128 rows: of 64 columns of h; of 128 of out (and of what the backward pass makes).  So 64 columns of h and 128 of out
+ * take 2^30 - 128 rows. */
 typedef struct rt_gated_ffn {
     int16_t dtype;               /* RT_F32 / RT_BF16 / RT_F16 */
     int16_t pre_dtype;           /* of pre_gate and pre_up: RT_F32 (0) or dtype */

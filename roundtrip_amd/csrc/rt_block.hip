@@ -44,6 +44,7 @@ struct DeviceScope {
 
 constexpr int64_t MAX_DIM = 1 << 20;              // elements of a row, and of its stride: a tile then spans < 2^31 bytes
 constexpr int64_t MAX_ROWS = 1ll << 40;
+constexpr int64_t MAX_TILES = (1 << 23) - 1;      // of up to 512 threads: a launch holds less than 2^32
 
 int elem_size(int dtype) { return dtype == RT_F32 ? 4 : 2; }
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
@@ -150,6 +151,7 @@ int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Pla
     for (int i = 0; i < (al && !f32 ? 3 : 2); ++i) {
         const Size& z = sizes[i];
         const int64_t m = (p.M + z.bm - 1) / z.bm, n = (p.N + z.cn - 1) / z.cn, tiles = m * n * p.nbatch;
+        if (m * n > MAX_TILES) continue;
         for (int64_t k = 1; k <= 32 && (k == 1 || (k * 2 <= steps && tiles * k <= 2 * cus)); k *= 2) {
             const int64_t per = (steps + k - 1) / k, load = (tiles * k + cus - 1) / cus;
             const double join = k > 1 ? 5.0 + (double)k * pl.nslot * p.M * pl.Np * 8 / 4.5e6 : 0.0;
@@ -164,7 +166,7 @@ int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Pla
             tn = n;
         }
     }
-    if (tm * tn > 0x7fffff || steps > 0x7fffffff)           // 512 threads a tile: a launch holds less than 2^32
+    if (tm == 0 || steps > 0x7fffffff)
         return failf(ctx, RT_EUNSUPPORTED, "a product of %lld x %d over %lld is larger than one launch covers", (long long)p.M, p.N,
                      (long long)p.K);
     pl.tiles_m = (int)tm;
@@ -222,7 +224,7 @@ struct Ffn {
     size_t pad_x, pad_in, pad_down, pad_dout;      // bytes of a copy, 0: none is needed
     Product gated, down;           // forward
     Product dh, dx, dw_in, dw_down;
-    size_t ws_fwd, ws_bwd, part_fwd, part_bwd;
+    size_t ws, part;               // bytes of the workspace, and of partial sums in it
 };
 
 constexpr int PAD_ROWS = 1024;
@@ -243,7 +245,8 @@ int most_part_bytes(rt_ctx* ctx, int cus, int dtype, const Product& p, size_t& m
     return RT_OK;
 }
 
-int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& f) {
+// The sizes, and the products and workspace of the forward or the backward pass.
+int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, bool backward, Ffn& f) {
     if (!in) return failf(ctx, RT_EINVAL, "%s: the arguments are NULL", fn);
     f.a = *in;
     rt_gated_ffn& a = f.a;
@@ -290,22 +293,19 @@ int ffn_make(rt_ctx* ctx, const char* fn, const rt_gated_ffn* in, int cus, Ffn& 
         f.down.wpad = f.dh.wpad = f.pad_down;
         f.dh.xpad = f.dw_down.wpad = f.pad_dout;
     }
-    f.ws_fwd = f.ws_bwd = 0;
+    f.ws = f.part = 0;
     if (a.T == 0) return RT_OK;
     // whichever kernels the call's alignment lets it use, with and without x_lo
-    size_t fwd = 0, bwd = 0;
-    int rc;
     Product other = f.gated;
     other.nseg = 3 - other.nseg;
-    for (const Product* p : {&f.gated, &other, &f.down})
-        if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, fwd))) return rc;
-    for (const Product* p : {&f.dh, &f.dx, &f.dw_in, &f.dw_down})
-        if ((rc = most_part_bytes(ctx, cus, a.dtype, *p, bwd))) return rc;
+    const Product* forward[] = {&f.gated, &other, &f.down};
+    const Product* back[] = {&f.dh, &f.dx, &f.dw_in, &f.dw_down};
+    for (int i = 0; i < (backward ? 4 : 3); ++i) {
+        const int rc = most_part_bytes(ctx, cus, a.dtype, backward ? *back[i] : *forward[i], f.part);
+        if (rc) return rc;
+    }
     const size_t copies = 2 * f.pad_x + 2 * f.pad_in + f.pad_down;      // (x_lo too)
-    f.ws_fwd = f.h_bytes + up(fwd, 256) + copies;
-    f.ws_bwd = 3 * f.h_bytes + up(bwd, 256) + copies + f.pad_dout;
-    f.part_fwd = fwd;
-    f.part_bwd = bwd;
+    f.ws = (backward ? 3 : 1) * f.h_bytes + up(f.part, 256) + copies + (backward ? f.pad_dout : 0);
     return RT_OK;
 }
 
@@ -363,7 +363,7 @@ int ffn_forward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, char* ws) {
     const int64_t es = f.es;
     char* h = ws;
     Operands o;
-    int rc = ffn_operands(ctx, v, f, nullptr, 0, ws + f.h_bytes + up(f.part_fwd, 256), o);
+    int rc = ffn_operands(ctx, v, f, nullptr, 0, ws + f.h_bytes + up(f.part, 256), o);
     if (rc) return rc;
     GemmArgs g;
     memset(&g, 0, sizeof g);
@@ -393,7 +393,7 @@ int ffn_backward(rt_ctx* ctx, const RtCtxView& v, const Ffn& f, const rt_gated_f
     g.act = a.act;
     g.alpha = a.alpha;
     Operands o;
-    int rc = ffn_operands(ctx, v, f, r.dout, r.ld_dout, ws + 3 * f.h_bytes + up(f.part_bwd, 256), o);
+    int rc = ffn_operands(ctx, v, f, r.dout, r.ld_dout, ws + 3 * f.h_bytes + up(f.part, 256), o);
     if (rc) return rc;
     // dh = dout Wd^T, and from it what the gate's and up's sums get, and h again
     set_x(g, o.dout, o.dout, o.ld_dout);
@@ -534,9 +534,9 @@ int rt_gated_ffn_workspace(rt_ctx* ctx, const rt_gated_ffn* a, int backward, siz
     RtCtxView v;
     rt_ctx_view(ctx, &v);
     Ffn f;
-    const int rc = ffn_make(ctx, "rt_gated_ffn_workspace", a, v.cu_count, f);
+    const int rc = ffn_make(ctx, "rt_gated_ffn_workspace", a, v.cu_count, backward != 0, f);
     if (rc) return rc;
-    *bytes = backward ? f.ws_bwd : f.ws_fwd;
+    *bytes = f.ws;
     return RT_OK;
 }
 
@@ -546,20 +546,20 @@ int rt_gated_ffn_dev(rt_ctx* ctx, const rt_gated_ffn* args, void* ws, size_t ws_
     RtCtxView v;
     rt_ctx_view(ctx, &v);
     Ffn f;
-    int rc = ffn_make(ctx, fn, args, v.cu_count, f);
+    int rc = ffn_make(ctx, fn, args, v.cu_count, false, f);
     if (rc) return rc;
     const rt_gated_ffn& a = f.a;
     const Mat in[] = {{"x", a.x, a.T, a.d_in, a.ldx, f.es}, {"w_gate", a.w_gate, a.d_in, a.d_ff, a.ld_in, f.es}, {"w_up", a.w_up, a.d_in, a.d_ff, a.ld_in, f.es},
                       {"w_down", a.w_down, a.d_ff, a.d_out, a.ld_down, f.es}, {"x_lo", a.x_lo, a.T, a.d_in, a.ldx, f.es}};
     const Mat out[] = {{"out", a.out, a.T, a.d_out, a.ld_out, f.es}, {"pre_gate", a.pre_gate, a.T, a.d_ff, a.ld_pre, f.kept},
-                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, f.kept}, {"the workspace", ws, 1, (int64_t)f.ws_fwd, (int64_t)f.ws_fwd, 1}};
+                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, f.kept}, {"the workspace", ws, 1, (int64_t)f.ws, (int64_t)f.ws, 1}};
     for (int i = 0; i < 5; ++i)
         if ((rc = check_mat(ctx, fn, in[i], i < 4))) return rc;
     for (int i = 0; i < 3; ++i)
         if ((rc = check_mat(ctx, fn, out[i], i == 0))) return rc;
     if (!a.pre_gate != !a.pre_up) return failf(ctx, RT_EINVAL, "%s: give both of pre_gate and pre_up, or neither", fn);
     if (a.T == 0) return RT_OK;
-    if ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_fwd)) || (rc = check_disjoint(ctx, fn, in, 5, out, 4))) return rc;
+    if ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws)) || (rc = check_disjoint(ctx, fn, in, 5, out, 4))) return rc;
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);
     return ffn_forward(ctx, v, f, (char*)ws);
@@ -572,7 +572,7 @@ int rt_gated_ffn_backward_dev(rt_ctx* ctx, const rt_gated_ffn* args, const rt_ga
     RtCtxView v;
     rt_ctx_view(ctx, &v);
     Ffn f;
-    int rc = ffn_make(ctx, fn, args, v.cu_count, f);
+    int rc = ffn_make(ctx, fn, args, v.cu_count, true, f);
     if (rc) return rc;
     const rt_gated_ffn& a = f.a;
     rt_gated_ffn_grads r = *grads;
@@ -585,12 +585,12 @@ int rt_gated_ffn_backward_dev(rt_ctx* ctx, const rt_gated_ffn* args, const rt_ga
                       {"pre_up", a.pre_up, a.T, a.d_ff, a.ld_pre, f.kept}, {"dout", r.dout, a.T, a.d_out, r.ld_dout, f.es}};
     const Mat out[] = {{"dx", r.dx, a.T, a.d_in, r.ld_dx, f.es}, {"dw_gate", r.dw_gate, a.d_in, a.d_ff, r.ld_dw_in, f.es},
                        {"dw_up", r.dw_up, a.d_in, a.d_ff, r.ld_dw_in, f.es}, {"dw_down", r.dw_down, a.d_ff, a.d_out, r.ld_dw_down, f.es},
-                       {"the workspace", ws, 1, (int64_t)f.ws_bwd, (int64_t)f.ws_bwd, 1}};
+                       {"the workspace", ws, 1, (int64_t)f.ws, (int64_t)f.ws, 1}};
     for (const Mat& m : in)
         if ((rc = check_mat(ctx, fn, m, true))) return rc;
     for (int i = 0; i < 4; ++i)
         if ((rc = check_mat(ctx, fn, out[i], false))) return rc;
-    if (a.T > 0 && ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws_bwd)))) return rc;
+    if (a.T > 0 && ((rc = check_ws(ctx, fn, ws, ws_bytes, f.ws)))) return rc;
     if ((rc = check_disjoint(ctx, fn, in, 7, out, a.T > 0 ? 5 : 4))) return rc;
     DeviceScope dev(v.device);
     HIPCHK(ctx, dev.err);
