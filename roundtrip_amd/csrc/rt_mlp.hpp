@@ -75,7 +75,7 @@ __device__ __forceinline__ float vmax(float a, float b) {
     return r;
 }
 
-// lrelu of accumulator registers [4q, 4q+4) of one tile, in place: max(t, alpha*t), two elements per v_pk_mul_f32.
+// lrelu of accumulator registers [4q, 4q+4) of one tile, in place: max(t, alpha*t), v_mul_f32 and v_max_f32 an element.
 __device__ __forceinline__ void lrelu_quad(f32x16& t, int q, float alpha) {
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
