@@ -207,28 +207,27 @@ def run(s):
     return _run_own(s) if own else _run_plain(s)
 
 
-def _tensors(v):
-    if isinstance(v, torch.Tensor):
-        yield v
-    elif isinstance(v, (dict, list, tuple)):
-        for x in v.values() if isinstance(v, dict) else v:
-            yield from _tensors(x)
+class _Held(object):
+    """Goes with its state, and waits then for the passes that use the state's arrays."""
+
+    def __init__(self, eng):
+        self.eng = eng
+
+    def __del__(self):
+        self.eng.sync()
 
 
 def _join_streams(s):
-    """The calls run on the engine's stream and the arrays are torch's; neither stream waits for the other by itself.  Before
-    a state's first pass: its inputs are there, and no array goes to another owner while a pass uses it.  Outputs are read when the
-    device, or the engine (`Engine.sync`), has been waited for."""
-    stream = torch.cuda.ExternalStream(s["eng"].stream)
-    stream.wait_stream(torch.cuda.current_stream())
-    for t in _tensors(s):
-        t.record_stream(stream)
-    s["joined"] = True
+    """The calls run on the engine's stream and the arrays are torch's; neither stream waits for the other by itself.  From a
+    state's first pass on: its inputs are there, and no array goes to another owner while a pass uses it.  Outputs are read when
+    the device, or the engine (`Engine.sync`), has been waited for."""
+    torch.cuda.ExternalStream(s["eng"].stream).wait_stream(torch.cuda.current_stream())
+    s["held"] = _Held(s["eng"])
 
 
 def _run_own(s):
     eng, case = s["eng"], s["case"]
-    if "joined" not in s:
+    if "held" not in s:
         _join_streams(s)
     ws, size = s["ws"].data_ptr(), s["ws"].numel()
     if case["op"] == "block":
