@@ -1,6 +1,7 @@
 """perf/operators.py as a program uses it: its arrays are torch's, its calls the engine's."""
 import importlib
 import os
+import subprocess
 import sys
 
 import pytest
@@ -68,3 +69,19 @@ def test_arrays_of_a_pass_under_way_go_to_nobody_else(engine, ops):
     for t in new:
         assert bool((t == 7.0).all())
     eng.sync()
+
+
+def test_a_program_that_ends_with_states_alive_ends_well(engine):
+    """In whatever order the interpreter lets go of the engine and of the states."""
+    code = ("import torch, perf.operators as p\n"
+            "p.own = True\n"
+            "c = %r\n"
+            "states = [p.prepare(c, i) for i in range(2)]\n"
+            "torch.cuda.synchronize()\n"
+            "outs = [p.run(s) for s in states]\n"
+            "torch.cuda.synchronize()\n"
+            "print('done', flush=True)\n" % (CASES[0],))
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.PIPE, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip() == b"done", (r.returncode, r.stdout[-500:], r.stderr[-2000:])
+    assert b"Exception ignored" not in r.stderr, r.stderr[-2000:]
