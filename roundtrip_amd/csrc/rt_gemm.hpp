@@ -9,7 +9,7 @@
 //
 // Bound by the matrix cores.  Measured, all launches of a call: 8192 rows of a 4096 x 16384 bf16 block 2.6 ms = 1.27 PF/s (a
 // library product of those sizes alone: 1.15 to 1.34); a training step at 4096 x 2048 x 8192 bf16 1.29 ms = 0.96 PF/s; 10000 x
-// 512 x 1024 float32 268 us = 117 TF/s (matrix cores busy 74 % and 65 % of the two products).
+// 512 x 1024 float32 269 us = 117 TF/s (matrix cores busy 74 % and 65 % of the two products).
 #pragma once
 #include "rt_elem.hpp"
 
@@ -53,34 +53,27 @@ __device__ __forceinline__ void put4(char* p, f32x4 v, int valid) {
 }
 
 // Four kept values as they lie in memory, of type KT.
-template <int KT> struct Kept {
-    typedef typename Elem<KT>::Quad Quad;
-    Quad v;
-    template <bool QUADS> __device__ __forceinline__ void load(const char* p, int valid) {
-        if (QUADS) {
-            v = *(const Quad*)p;
-        } else {
-            const f32x4 f = load4<KT>(p, valid);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = (typename Elem<KT>::T)f[j];       // from that type, so exact
-        }
-    }
-};
+template <int KT> using Kept = typename Elem<KT>::Quad;
+template <int KT, bool QUADS>
+__device__ __forceinline__ Kept<KT> load_kept(const char* p, int valid) {
+    if (QUADS) return *(const Kept<KT>*)p;
+    return __builtin_convertvector(load4<KT>(p, valid), Kept<KT>);       // of that type, so exact
+}
 
 // The kept gate and up at four places (columns behind N: zeros).
 template <int KT, bool QUADS>
 __device__ __forceinline__ void kept4(const GemmArgs& a, long long m, int n, Kept<KT>& g, Kept<KT>& u) {
     const int valid = a.N - n;
-    g.v = u.v = typename Kept<KT>::Quad{0, 0, 0, 0};
+    g = u = Kept<KT>{0, 0, 0, 0};
     if (valid <= 0) return;
-    const long long at = m * a.lde + (long long)n * ES<KT>;
-    g.template load<QUADS>(a.e[0] + at, valid);
-    u.template load<QUADS>(a.e[1] + at, valid);
+    const char *pg = a.e[0] + m * a.lde + (long long)n * ES<KT>, *pu = a.e[1] + m * a.lde + (long long)n * ES<KT>;
+    g = load_kept<KT, QUADS>(pg, valid);
+    u = load_kept<KT, QUADS>(pu, valid);
 }
 
 // EPI_GATED_BWD: v is dh.
 template <int DT, int ACT, bool QUADS, int KT>
-__device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int n, f32x4 v, const Kept<KT>& kept_g, const Kept<KT>& kept_u) {
+__device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int n, f32x4 v, Kept<KT> g, Kept<KT> u) {
     const int room = a.No - n, valid = a.N - n;
     if (room <= 0) return;
     const long long c = (long long)n * ES<DT>;
@@ -88,12 +81,11 @@ __device__ __forceinline__ void epilogue_bwd(const GemmArgs& a, long long m, int
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float t, d;
-        const float u = (float)kept_u.v[j];
-        act_f<DT, ACT>(a.alpha, (float)kept_g.v[j], t, d);
+        act_f<DT, ACT>(a.alpha, (float)g[j], t, d);
         const float w = j < valid ? v[j] : 0.0f;         // zeros behind the row's end, whatever the sum there was of
-        dg[j] = w * u * d;
+        dg[j] = w * (float)u[j] * d;
         du[j] = w * t;
-        h[j] = t * u;
+        h[j] = t * (float)u[j];
     }
     put4<DT, QUADS>(a.o[0] + m * a.ldo[0] + c, dg, room);
     put4<DT, QUADS>(a.o[1] + m * a.ldo[1] + c, du, room);

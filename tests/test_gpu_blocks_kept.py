@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 # few rows (vector and matrix units, K split), tiles of 64, 128 and 256, with K in one run and in several, odd widths, copies of them
 SIZES = [(1, 64, 128, 64), (3, 2000, 96, 5), (17, 3000, 260, 128), (33, 100, 72, 40), (300, 512, 65, 31), (67, 528, 1344, 48), (1030, 101, 203, 77),
-         (3397, 136, 1168, 40), (130, 3488, 2056, 456), (4033, 45, 2184, 140), (1000, 40, 2051, 1200)]
+         (3397, 136, 1168, 40), (130, 3488, 2056, 456), (4033, 45, 2184, 140), (1000, 40, 2051, 1200), (931, 55, 2479, 145)]
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
