@@ -137,6 +137,7 @@ int plan_product(rt_ctx* ctx, int cus, int dtype, const Product& p, bool al, Pla
     // workgroups.  With L workgroups side by side on a CU (at most `fit`, what its LDS holds) a step (128 bytes of k) takes the
     // larger of `least`, what one workgroup waits for memory and barriers, and L * `each`, what the matrix core (16-bit tiles
     // below 256: LDS) needs; splits are joined by another launch, which reads what they wrote.  By measurement, in us:
+    // (of long sums; the epilogue's bytes are not in it: where those count, products take up to twice what this says)
     //   16-bit: 256 x 256 1.65 / 1.65;  128 x 128 0.7 / 0.5;  64 x 64 0.7 / 0.25        float32: 128 x 128 2.2 / 1.9;  64 x 64 0.8 / 0.5
     struct Size { int bm, cn, fit; double least, each; };
     const int half = p.epi == EPI_GATED ? 2 : 1;

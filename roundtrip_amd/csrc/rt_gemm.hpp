@@ -9,7 +9,7 @@
 //
 // Bound by the matrix cores.  Measured, all launches of a call: 8192 rows of a 4096 x 16384 bf16 block 2.6 ms = 1.27 PF/s (a
 // library product of those sizes alone: 1.15 to 1.34); a training step at 4096 x 2048 x 8192 bf16 1.29 ms = 0.96 PF/s; 10000 x
-// 512 x 1024 float32 269 us = 117 TF/s (matrix cores busy 74 % and 65 % of the two products).
+// 512 x 1024 float32 268 us = 117 TF/s (matrix cores busy 74 % and 65 % of the two products).
 #pragma once
 #include "rt_elem.hpp"
 
