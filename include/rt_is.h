@@ -357,7 +357,8 @@ int rt_gated_ffn_backward_dev(rt_ctx* ctx, const rt_gated_ffn* args, const rt_ga
  * N(v; w) = RT_NORM_*(v) * (w + w_offset); a NULL w counts as ones, without the offset.  Without a branch y = res_scale x
  * (the norm before a block: x and n alone).  Row t uses row t / rows_per_gate of gate: 1 is a gate for every row, T one for
  * all, a sequence length one for each sequence (the last group may be short); a NULL gate counts as ones.
- * n is made of the unrounded y. */
+ * n is made of the unrounded y.  Squares are summed in float32: a row of values beyond some 1e19 has an infinite sum and is
+ * normed to zeros. */
 typedef struct rt_block_norm {
     int32_t dtype, kind;         /* RT_NORM_* */
     int32_t d;                   /* 1 .. 32768 (RT_F32: 16384) */
@@ -390,7 +391,7 @@ int rt_block_norm_workspace(rt_ctx* ctx, const rt_block_norm* args, size_t* byte
 int rt_block_norm_dev(rt_ctx* ctx, const rt_block_norm* args);
 
 /* Backward, at the branch, y, gate and weights of a forward call; x and n are not read (without a branch and without a y, x
- * is read in y's place). */
+ * is read in y's place).  In 16 bits y is the rounded one: its half step is in the gradients that go through n. */
 int rt_block_norm_backward_dev(rt_ctx* ctx, const rt_block_norm* args, const rt_block_norm_grads* grads, void* ws,
                                size_t ws_bytes);
 
